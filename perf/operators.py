@@ -1,0 +1,382 @@
+"""The operators of a residual block's training path that are measured: 8-bit activation checkpoints, what the backward pass
+reads back from them, the weight gradient formed from them, and the norms around a block fused with its gate and residual scale.
+
+Maps are channels-last, (n, h, w, c).  A checkpoint of a map holds e4m3 codes of the map's shape and one byte per 32 channels, the
+biased exponent of the group's scale."""
+import math
+
+import torch
+
+own = False
+
+DEV = "cuda"
+TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
+GROUP = 32        # channels that share a scale
+BIAS, LOWEST = 127, 10   # exponent byte of scale 1; the lowest exponent byte that a checkpoint holds
+
+
+def listed():
+    return [
+        # saving a 64-channel ReLU map of four 1024 x 1024 training crops, with the ReLU pattern for the data gradient
+        {"name": "pack_crops64", "op": "pack", "n": 4, "h": 1024, "w": 1024, "c": 64, "dtype": "bf16", "bits": True},
+        # saving fp32 G-buffers: ten channels, an odd width
+        {"name": "pack_gbuffers10_f32", "op": "pack", "n": 2, "h": 540, "w": 959, "c": 10, "dtype": "f32", "bits": False},
+        # bringing back the widest map of the temporal network's fusion stage, for eight crops
+        {"name": "restore_wide256", "op": "restore", "n": 8, "h": 272, "w": 480, "c": 256, "dtype": "bf16"},
+        # the ReLU of a saved 64-channel map applied to a gradient
+        {"name": "mask_crops64", "op": "mask", "n": 4, "h": 1024, "w": 1024, "c": 64, "dtype": "bf16"},
+        # the layer most of the default network's training step goes to, on four crops
+        {"name": "wgrad3_crops64", "op": "wgrad", "n": 4, "h": 1024, "w": 1024, "c": 64, "cout": 64, "k": 3},
+        # a pointwise layer of the temporal network's encoder at a quarter of the resolution, odd height
+        {"name": "wgrad1_wide160", "op": "wgrad", "n": 2, "h": 135, "w": 240, "c": 160, "cout": 112, "k": 1},
+        # one row: a conditioning vector through the norms around a block
+        {"name": "norm_row2048", "op": "norm", "n": 1, "h": 1, "w": 1, "c": 2048, "dtype": "bf16", "kind": "rms", "gate": "channel", "act": "none", "learned": False, "post": True, "pre": True},
+        # a residual block of the 64-channel trunk on four crops, each crop with gates of its own
+        {"name": "norm_crops64", "op": "norm", "n": 4, "h": 1024, "w": 1024, "c": 64, "dtype": "bf16", "kind": "layer", "gate": "sample", "act": "sigmoid", "learned": True, "post": True, "pre": True},
+        # full precision, odd sizes, a gate for every element
+        {"name": "norm_odd99_f32", "op": "norm", "n": 3, "h": 135, "w": 241, "c": 99, "dtype": "f32", "kind": "layer", "gate": "map", "act": "sigmoid", "learned": False, "post": True, "pre": True},
+        # the backward pass of a few rows, where launches count
+        {"name": "norm_bwd_rows4", "op": "norm_bwd", "n": 1, "h": 1, "w": 4, "c": 1024, "dtype": "f32", "kind": "layer", "gate": "none", "act": "none", "learned": False, "post": True, "pre": True, "saved": "map"},
+        # the trunk's block again, its saved maps held as checkpoints
+        {"name": "norm_bwd_crops64_saved8", "op": "norm_bwd", "n": 4, "h": 1024, "w": 1024, "c": 64, "dtype": "bf16", "kind": "layer", "gate": "sample", "act": "sigmoid", "learned": True, "post": True, "pre": True, "saved": "checkpoint"},
+        # wide rows, scaled by channel
+        {"name": "norm_bwd_wide4096", "op": "norm_bwd", "n": 1, "h": 64, "w": 250, "c": 4096, "dtype": "bf16", "kind": "rms", "gate": "channel", "act": "none", "learned": True, "post": True, "pre": True, "saved": "map"},
+    ]
+
+
+def draw(rng):
+    op = rng.choice(["pack", "pack", "restore", "mask", "wgrad", "wgrad", "norm", "norm", "norm_bwd", "norm_bwd"])
+    spread = lambda lo, hi: min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 1)))))))  # noqa: E731
+    if op == "wgrad":
+        c, cout = 16 * spread(1, 16), 16 * spread(1, 12)
+        most = (1 << 27) // (c * cout)
+    else:
+        low = 16 if op.startswith("norm") else 1
+        c = 64 if rng.random() < 0.3 else spread(low, 320) if rng.random() < 0.7 or low == 1 else spread(321, 8192)
+        most = (1 << 26) // c
+    n = rng.randint(1, 4)
+    h = spread(1, max(1, min(1080, most // n)))
+    w = spread(1, max(1, min(1920, most // (n * h))))
+    case = {"op": op, "n": n, "h": h, "w": w, "c": c}
+    if op == "wgrad":
+        case.update(cout=cout, k=rng.choice([1, 3]))
+        return case
+    case["dtype"] = "bf16" if op == "mask" else rng.choice(["bf16", "bf16", "f32"])
+    if op == "pack":
+        case["bits"] = c == 64 and case["dtype"] == "bf16" and rng.random() < 0.5
+    if op.startswith("norm"):
+        case.update(kind=rng.choice(["layer", "rms"]), gate=rng.choice(["none", "channel", "sample", "map"]), act=rng.choice(["none", "sigmoid"]),
+                    learned=rng.random() < 0.5)
+        case.update(zip(("post", "pre"), rng.choice([(True, True), (True, True), (True, False), (False, True)])))
+        if op == "norm_bwd":
+            case["saved"] = rng.choice(["map", "checkpoint"])
+    return case
+
+
+# ---------------------------------------------------------------------------------------------------------------- inputs
+
+def _exponents(amax):
+    """The exponent byte of a group whose largest magnitude is amax (fp32): the smallest scale that brings it to 448 or less."""
+    b = amax.view(torch.int32)
+    return ((b >> 23) - 8 + ((b & 0x7FFFFF) > 0x600000).int()).clamp(min=LOWEST)
+
+
+def _spread(s, c):
+    """Values by group -> values by channel."""
+    return s.repeat_interleave(GROUP, dim=-1)[..., :c]
+
+
+def _encode(x):
+    """Codes and exponent bytes of a map."""
+    c = x.shape[-1]
+    g = -(-c // GROUP)
+    f = x.float()
+    f = torch.where(f.isfinite(), f, torch.nan)
+    amax = torch.nn.functional.pad(f.abs().nan_to_num(0.0), (0, g * GROUP - c)).unflatten(-1, (g, GROUP)).amax(-1)
+    e = _exponents(amax)
+    codes = (f * _spread(_power(2 * BIAS - e), c)).to(torch.float8_e4m3fn)
+    lost = (codes.view(torch.uint8) & 0x7F == 0) & (f != 0)
+    codes = torch.where(lost, codes.view(torch.uint8) | 1, codes.view(torch.uint8)).view(torch.float8_e4m3fn)
+    return codes, e.to(torch.uint8)
+
+
+def _power(e):
+    """2^(e - 127) in fp32 for whole e from 1 to 254."""
+    return (e.int() << 23).view(torch.float32)
+
+
+def _decode(codes, scales):
+    return codes.float() * _spread(_power(scales), codes.shape[-1])
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    n, h, w, c = (case[k] for k in "nhwc")
+    shape = (n, h, w, c)
+
+    def normal(*s, scale=1.0, dtype=torch.float32):
+        return (torch.randn(s, device=DEV, generator=g) * scale).to(dtype)
+
+    def activations(dtype, relu=True):
+        """A map as a layer leaves it: channels of different size, behind a ReLU or not."""
+        a = torch.randn(shape, device=DEV, generator=g) * torch.exp(normal(c))
+        return (a.relu() if relu else a + 0.3 * normal(c)).to(dtype)
+
+    if case["op"] == "pack":
+        return {"case": case, "x": activations(TYPES[case["dtype"]])}
+    if case["op"] == "restore":
+        return {"case": case, "saved": _encode(activations(TYPES[case["dtype"]], relu=False))}
+    if case["op"] == "mask":
+        return {"case": case, "saved": _encode(activations(torch.bfloat16)), "dy": normal(*shape, scale=1e-4, dtype=torch.bfloat16)}
+    if case["op"] == "wgrad":
+        dz = normal(n, h, w, case["cout"], scale=1e-4)
+        dz = torch.where(normal(n, h, w, case["cout"]) > 0, dz, 0.0)   # behind a ReLU: half of them are zero
+        return {"case": case, "saved": _encode(activations(torch.bfloat16)), "dz": dz.bfloat16()}
+    t = TYPES[case["dtype"]]
+    s = {"case": case, "h": activations(t, relu=False), "post": None, "pre": None, "gate": None, "scale": 0.2}
+    for k in ("post", "pre"):
+        if case[k]:
+            s[k] = (1 + normal(c, scale=0.2), normal(c, scale=0.2) if case["kind"] == "layer" else None)
+    if case["gate"] != "none":
+        s["gate"] = {"channel": lambda: normal(c), "sample": lambda: normal(n, c), "map": lambda: normal(*shape, dtype=t)}[case["gate"]]()
+    if case["learned"]:
+        s["scale"] = torch.full((), 0.2, device=DEV) + 0.05 * torch.rand((), device=DEV, generator=g)
+    if case["op"] == "norm":
+        s["x"] = normal(*shape, scale=2.0, dtype=t)
+        return s
+    s["r"] = (2 * torch.randn(shape, device=DEV, generator=g) + 0.3 * s["h"].float()).to(t)
+    s["dr"] = ((torch.randn(shape, device=DEV, generator=g) + 0.3 * torch.tanh(s["h"].float())) * 1e-2).to(t)
+    s["dn"] = normal(*shape, scale=1e-2, dtype=t) if case["pre"] else None
+    if case["saved"] == "checkpoint":
+        s["h"], s["r"] = _encode(s["h"]), _encode(s["r"])
+    return s
+
+
+# ---------------------------------------------------------------------------------------------------------------- one pass
+
+def run(state):
+    return (_own if own else _plain)(state)
+
+
+def _own(s):
+    from superresolution_amd import functional as F
+    case = s["case"]
+    held = lambda v, t: F.Checkpoint8(v[0], v[1], t) if isinstance(v, tuple) else v  # noqa: E731
+    if case["op"] == "pack":
+        ck = F.checkpoint8_pack(s["x"], signbits=case["bits"])
+        return (ck.codes, ck.scales) + ((ck.signbits,) if case["bits"] else ())
+    if case["op"] == "restore":
+        return F.checkpoint8_restore(held(s["saved"], TYPES[case["dtype"]]))
+    if case["op"] == "mask":
+        return F.relu_mask(s["dy"], held(s["saved"], torch.bfloat16))
+    if case["op"] == "wgrad":
+        return F.checkpoint8_wgrad(held(s["saved"], torch.bfloat16), s["dz"], case["c"], case["cout"], case["k"])
+    how = dict(post=s["post"], gate=s["gate"], scale=s["scale"], pre=s["pre"], kind=case["kind"], gate_act=case["act"])
+    if case["op"] == "norm":
+        return F.norm_residual(s["x"], s["h"], **how)
+    t = TYPES[case["dtype"]]
+    return tuple(F.norm_residual_bwd(held(s["h"], t), held(s["r"], t), s["dr"], s["dn"], **how))
+
+
+def _plain(s):
+    case = s["case"]
+    if case["op"] == "pack":
+        codes, scales = _encode(s["x"])
+        return (codes, scales) + ((_pattern(s["x"] > 0),) if case["bits"] else ())
+    if case["op"] == "restore":
+        return _decode(*s["saved"]).to(TYPES[case["dtype"]])
+    if case["op"] == "mask":
+        return torch.where(s["saved"][0].float() > 0, s["dy"].float(), 0.0).bfloat16()
+    if case["op"] == "wgrad":
+        return _plain_wgrad(_decode(*s["saved"]), s["dz"].float(), case["k"])
+    return _plain_norm(s) if case["op"] == "norm" else _plain_norm_bwd(s)
+
+
+def _pattern(positive):
+    """The ReLU pattern of a 64-channel map as 1 bit per element: word (x % 8) * 8 + channel // 8 of 32 pixels of a row
+    holds channel % 8 of the pixels x % 8, x % 8 + 8, ... in its four bytes."""
+    n, h, w, _ = positive.shape
+    g = -(-w // 32)
+    p = torch.nn.functional.pad(positive, (0, 0, 0, g * 32 - w)).view(n, h, g, 4, 8, 8, 8)    # n h g x//8 x%8 c//8 c%8
+    p = p.permute(0, 1, 2, 4, 5, 3, 6).reshape(n, h, g, 64, 32)
+    place = torch.arange(32, device=p.device)
+    return (p.long() << place).sum(-1).to(torch.int32)   # bit 31 wraps to the sign
+
+
+def _plain_wgrad(x, dz, k):
+    n, h, w, c = x.shape
+    cout = dz.shape[-1]
+    if k == 3:
+        x = torch.nn.functional.pad(x, (0, 0, 1, 1, 1, 1)).unfold(1, 3, 1).unfold(2, 3, 1)    # n h w c ky kx
+    # one product per row of the map, then the sum of them
+    dw = torch.bmm(dz.view(n * h, w, cout).transpose(1, 2).contiguous(), x.reshape(n * h, w, c * k * k)).sum(0)
+    return dw.view(cout, c, k, k), dz.sum((0, 1, 2))
+
+
+def _plain_statistics(v, kind, eps=1e-6):
+    mean = v.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(v[..., :1])
+    return mean, 1 / torch.sqrt((v - mean).square().mean(-1, keepdim=True) + eps)
+
+
+def _plain_affine(v, wb):
+    return v * wb[0] if wb[1] is None else v * wb[0] + wb[1]
+
+
+def _plain_gate(s):
+    """The gate as it multiplies a map, before and behind its activation."""
+    case, gate = s["case"], s["gate"]
+    if gate is None:
+        return None, 1.0
+    gate = gate.float()
+    gate = gate.view(case["n"], 1, 1, case["c"]) if case["gate"] == "sample" else gate
+    return gate, 1 / (1 + torch.exp(-gate)) if case["act"] == "sigmoid" else gate
+
+
+def _plain_norm(s):
+    case = s["case"]
+    h, t = s["h"].float(), s["x"].dtype
+    if s["post"] is not None:
+        mean, rstd = _plain_statistics(h, case["kind"])
+        h = _plain_affine((h - mean) * rstd, s["post"])
+    r = s["x"].float() + s["scale"] * _plain_gate(s)[1] * h
+    if s["pre"] is None:
+        return r.to(t), None
+    mean, rstd = _plain_statistics(r, case["kind"])
+    return r.to(t), _plain_affine((r - mean) * rstd, s["pre"]).to(t)
+
+
+def _plain_norm_bwd(s):
+    case, t, rows = s["case"], s["dr"].dtype, (0, 1, 2)
+    h, r = (_decode(*v) if isinstance(v, tuple) else v.float() for v in (s["h"], s["r"]))
+    layer = case["kind"] == "layer"
+
+    def through(v, d, wb):
+        """Gradients of a norm: of its input, weight and bias."""
+        mean, rstd = _plain_statistics(v, case["kind"])
+        hat, u = (v - mean) * rstd, d * wb[0]
+        dv = u - hat * (u * hat).mean(-1, keepdim=True) - (u.mean(-1, keepdim=True) if layer else 0.0)
+        return hat, rstd * dv, (d * hat).sum(rows), d.sum(rows) if layer else None
+
+    dx, pre_w, pre_b = s["dr"].float(), None, None
+    if s["pre"] is not None:
+        _, d, pre_w, pre_b = through(r, s["dn"].float(), s["pre"])
+        dx = dx + d
+    gate, g = _plain_gate(s)
+    dp = s["scale"] * g * dx
+    p, dh, post_w, post_b = h, dp, None, None
+    if s["post"] is not None:
+        hat, dh, post_w, post_b = through(h, dp, s["post"])
+        p = _plain_affine(hat, s["post"])
+    dgate = None
+    if gate is not None:
+        dgate = s["scale"] * dx * p
+        dgate = dgate.sum(rows) if case["gate"] == "channel" else dgate.sum((1, 2)) if case["gate"] == "sample" else dgate
+        if case["act"] == "sigmoid":
+            g1 = g.reshape(dgate.shape)
+            dgate = dgate * g1 * (1 - g1)
+        dgate = dgate.to(s["gate"].dtype)
+    dscale = (dx * g * p).sum() if case["learned"] else None
+    return dx.to(t), dh.to(t), post_w, post_b, dgate, dscale, pre_w, pre_b
+
+
+# ---------------------------------------------------------------------------------------------------------------- 64 bits
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    D = torch.float64
+    value = lambda v: torch.ldexp(v[0].to(D), (_spread(v[1], v[0].shape[-1]).to(D) - BIAS)) if isinstance(v, tuple) else v.to(D)  # noqa: E731
+    if case["op"] == "pack":
+        x, c = s["x"].to(D), case["c"]
+        parts = x.split(GROUP, dim=-1)
+        tops = torch.stack([p.abs().amax(-1) for p in parts], -1)
+        mantissa, power = torch.frexp(tops)                    # mantissa in [1/2, 1)
+        e = torch.where(mantissa > 0.875, power - 8, power - 9)
+        e = torch.where(tops > 0, e, LOWEST - BIAS).clamp(min=LOWEST - BIAS)
+        codes = torch.cat([torch.ldexp(p, -e[..., i:i + 1].to(D)) for i, p in enumerate(parts)], -1)
+        if not case["bits"]:
+            return codes, (e + BIAS).to(torch.uint8)
+        n, h, w, _ = x.shape
+        words = torch.zeros((n, h, (w + 31) // 32, 64), dtype=torch.int64, device=x.device)
+        for px in range(32):
+            on = (x[:, :, px::32] > 0).long()
+            for j in range(8):
+                words[:, :, :on.shape[2], px % 8 * 8:px % 8 * 8 + 8] += on[..., j::8] << (px // 8 * 8 + j)
+        return codes, (e + BIAS).to(torch.uint8), torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+    if case["op"] == "restore":
+        return value(s["saved"])
+    if case["op"] == "mask":
+        return s["dy"].to(D) * (value(s["saved"]) > 0)
+    if case["op"] == "wgrad":
+        x, dz, k = value(s["saved"]), s["dz"].to(D), case["k"]
+        n, h, w, c = x.shape
+        dw = torch.zeros((case["cout"], c, k, k), dtype=D, device=x.device)
+        for i in range(n):
+            for ky in range(k):
+                for kx in range(k):
+                    oy, ox = ky - k // 2, kx - k // 2
+                    a = x[i, max(0, oy):h + min(0, oy), max(0, ox):w + min(0, ox)]
+                    b = dz[i, max(0, -oy):h + min(0, -oy), max(0, -ox):w + min(0, -ox)]
+                    step = max(1, 65536 // max(1, b.shape[1]))
+                    for y in range(0, a.shape[0], step):
+                        dw[:, :, ky, kx] += b[y:y + step].reshape(-1, case["cout"]).T @ a[y:y + step].reshape(-1, c)
+        return dw, dz.sum((0, 1, 2))
+
+    leaf = lambda v: v.detach().to(D).requires_grad_()  # noqa: E731
+
+    def norm(v, w, b):
+        if case["kind"] == "layer":
+            out = (v - v.mean(-1, keepdim=True)) / torch.sqrt(v.var(-1, unbiased=False, keepdim=True) + 1e-6) * w
+            return out + b
+        return v / torch.sqrt((v * v).sum(-1, keepdim=True) / v.shape[-1] + 1e-6) * w
+
+    wb = {k: [None if v is None else leaf(v) for v in s[k]] if s[k] is not None else None for k in ("post", "pre")}
+    gate = None if s["gate"] is None else leaf(s["gate"])
+    scale = leaf(s["scale"]) if case["learned"] else torch.tensor(s["scale"], dtype=D, device=DEV)
+    h = value(s["h"]).requires_grad_(case["op"] == "norm_bwd")
+
+    def branch():
+        p = h if wb["post"] is None else norm(h, *wb["post"])
+        if gate is not None:
+            g = gate[:, None, None] if case["gate"] == "sample" else gate
+            p = p * (torch.sigmoid(g) if case["act"] == "sigmoid" else g)
+        return scale * p
+
+    if case["op"] == "norm":
+        with torch.no_grad():
+            r = s["x"].to(D) + branch()
+            return r, None if wb["pre"] is None else norm(r, *wb["pre"])
+    dx = s["dr"].to(D)
+    if wb["pre"] is not None:
+        r = value(s["r"]).requires_grad_()
+        norm(r, *wb["pre"]).backward(s["dn"].to(D))
+        dx = dx + r.grad
+        del r
+    branch().backward(dx)
+    of = lambda v: None if v is None else v.grad  # noqa: E731
+    post, pre = wb["post"] or (None, None), wb["pre"] or (None, None)
+    return dx, h.grad, of(post[0]), of(post[1]), of(gate), of(scale) if case["learned"] else None, of(pre[0]), of(pre[1])
+
+
+# ---------------------------------------------------------------------------------------------------------------- the least
+
+def work(case):
+    c, rows = case["c"], case["n"] * case["h"] * case["w"]
+    size = {"bf16": 2, "f32": 4}[case.get("dtype", "bf16")]
+    held = rows * (c + -(-c // GROUP))                                 # a checkpoint's bytes
+    if case["op"] == "pack":
+        bits = case["n"] * case["h"] * -(-case["w"] // 32) * 256 if case["bits"] else 0
+        return {"bytes": rows * c * size + held + bits, "flops": rows * c * 2}
+    if case["op"] == "restore":
+        return {"bytes": held + rows * c * size, "flops": rows * c}
+    if case["op"] == "mask":
+        return {"bytes": rows * c * 5, "flops": rows * c}
+    if case["op"] == "wgrad":
+        weight = case["cout"] * c * case["k"] ** 2
+        return {"bytes": held + rows * case["cout"] * 2 + 4 * (weight + case["cout"]), "flops": 2 * rows * weight}
+    gates = {"none": 0, "channel": 4 * c, "sample": 4 * c * case["n"], "map": rows * c * size}[case["gate"]]
+    params = 4 * c * (case["post"] + case["pre"]) * (2 if case["kind"] == "layer" else 1)
+    if case["op"] == "norm":
+        return {"bytes": rows * c * size * (3 + case["pre"]) + gates + params, "flops": rows * c * 16}
+    saved = held if case["saved"] == "checkpoint" else rows * c * size
+    reads = saved * (1 + case["pre"]) + rows * c * size * (1 + case["pre"])
+    return {"bytes": reads + 2 * rows * c * size + 2 * (gates + params), "flops": rows * c * 40}
