@@ -38,6 +38,7 @@ typedef enum {
 typedef enum { SRHIP_ACT_NONE = 0, SRHIP_ACT_RELU = 1, SRHIP_ACT_LRELU = 2 } srhip_act;
 typedef enum { SRHIP_BILINEAR = 0, SRHIP_NEAREST = 1 } srhip_interp;
 typedef enum { SRHIP_RES_ADD = 0, SRHIP_RES_MASK = 1, SRHIP_RES_PRE = 2 } srhip_res_mode;
+typedef enum { SRHIP_DT_BF16 = 0, SRHIP_DT_F32 = 1 } srhip_dtype;
 typedef enum { SRHIP_AUX_NONE = 0, SRHIP_AUX_EMIT = 1, SRHIP_AUX_MASKBITS = 2, SRHIP_AUX_DUALBITS = 3 } srhip_aux_mode;
 
 SRHIP_API int srhip_version(void);
@@ -584,6 +585,99 @@ SRHIP_API int srhip_layernorm_cf_bwd_f32(const float* x, const float* weight, co
 SRHIP_API int srhip_layernorm_cf_bwd_f32_static(const float* x, const float* weight, const float* dy, float* dx,
                                                 float* dweight, float* dbias, int n, int c, int hw, float eps,
                                                 void* stream);
+
+/* ---------------------------------------------------------------------------
+ * 8-bit activation checkpoints: what a training step keeps of a map for its backward pass (the maps that autograd saves for
+ * loss.backward(), core/trainer.py:160).  A row of c channels (a pixel of an NHWC map, or any row of a matrix) is held as c
+ * e4m3 codes and ceil(c / 32) bytes, one per 32 channels: s stands for the scale 2^(s - 127), 10 <= s <= 246, the smallest
+ * power of two that brings the group's largest finite magnitude to 448 or less (one above 1.75 * 2^127 is kept as that).  code = x / scale, rounded to nearest even;
+ * a value that is not 0 keeps a code that is not 0 (so [code > 0] is the ReLU pattern of a finite x); infinities and NaN
+ * become NaN.  A decoded value is exact in bf16 and fp32.
+ * Rows are contiguous; any c >= 1 and any alignment of the element type; rows == 0 does nothing.
+ * ------------------------------------------------------------------------- */
+SRHIP_API int srhip_checkpoint8_pack(const void* x, int dtype /* SRHIP_DT_* */, void* codes, void* scales, long long rows, int c, void* stream);
+/* The same for an (n, h, w, 64) bf16 map, also writing its ReLU pattern as srhip_signbits_from_map_bf16 does
+ * (srhip_conv3x3_signbits_bytes(n, h, w) bytes). */
+SRHIP_API int srhip_checkpoint8_pack_signbits(const void* x, void* codes, void* scales, void* signbits, int n, int h, int w, void* stream);
+SRHIP_API int srhip_checkpoint8_restore(const void* codes, const void* scales, void* y, int dtype, long long rows, int c, void* stream);
+/* out = dy where the code is a positive number, else 0 (bf16; out may be dy). */
+SRHIP_API int srhip_relu_mask_checkpoint8(const void* dy, const void* codes, void* out, size_t n, void* stream);
+
+/* Weight and bias gradient of a 3x3 (ksize 3) or 1x1 (ksize 1) layer whose input was kept as a checkpoint: the jobs of
+ * srhip_conv3x3_wgrad_multi / srhip_conv1x1_wgrad_multi with x = codes and, per job, x_scales[j] = the scale bytes
+ * (host array of device pointers).  x_cstride and x_coff are multiples of 16, codes start at a multiple of 16 bytes.  The result
+ * is that of the same call on the restored map, bit for bit. */
+SRHIP_API int srhip_conv_wgrad_checkpoint8(const srhip_wgrad_job* jobs, const void* const* x_scales, int njobs, void* workspace, int n, int h,
+                                           int w, int ci_pad, int co_pad, int w_i, int ksize, int accumulate, float scale, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The norms around a residual block, fused with its gate and residual scale, over `rows` contiguous rows of c channels:
+ *   p = N_post(h) (or h),   r = x + s * act(gate) * p,   n = N_pre(r)
+ * (LayerNorm core/arch/CAMixerSR.py:29-37 over the channels; gate core/arch/RepRFN.py:233-235; scaled residual sum
+ * core/models/model.py:33, with a trained scale core/models/model_final.py:256-258.)
+ *   x, h, r, n   bf16 or fp32 (dtype); h NULL: r = x, only n is written (no gate, no post norm)
+ *   post, pre    0 / 1: whether there is that norm; weights fp32[c], biases fp32[c] or NULL
+ *   kind         SRHIP_NORM_LAYER: (v - mean) / sqrt(var + eps) * w + b;  SRHIP_NORM_RMS: v / sqrt(mean v^2 + eps) * w + b
+ *   gate         SRHIP_GATE_ROWS: fp32 (rows / rows_per_gate, c), row i uses gate i / rows_per_gate (rows_per_gate = rows: one
+ *                vector for all);  SRHIP_GATE_MAP: (rows, c) of the maps' type, or fp32 with gate_f32
+ *   scale_ptr    fp32 on the device, or NULL: `scale`
+ * 1 <= c <= SRHIP_NORM_MAX_C.  n is the norm of the sum before it is rounded to r.  Outputs may alias no input. */
+typedef enum { SRHIP_NORM_LAYER = 0, SRHIP_NORM_RMS = 1 } srhip_norm_kind;
+typedef enum { SRHIP_GATE_NONE = 0, SRHIP_GATE_ROWS = 1, SRHIP_GATE_MAP = 2 } srhip_gate_mode;
+#define SRHIP_NORM_MAX_C 8192
+typedef struct {
+    const void* x;
+    const void* h;
+    const void* gate;
+    const float* post_weight;
+    const float* post_bias;
+    const float* pre_weight;
+    const float* pre_bias;
+    const float* scale_ptr;
+    void* r;
+    void* n;
+    long long rows, rows_per_gate;
+    int c, dtype, kind, post, pre, gate_mode, gate_f32, gate_sigmoid;
+    float scale, eps;
+} srhip_norm_residual_args;
+SRHIP_API int srhip_norm_residual_fwd(const srhip_norm_residual_args* args, void* stream);
+/* Its backward, from h, the sum r and the gradients of r and n; every gradient is written, none accumulated.
+ *   h, r         maps of the type `dtype`, or checkpoints: codes, with h_scales / r_scales their scale bytes (NULL: a map).  h
+ *                may be NULL where no post norm, gate or scale gradient asks for it; r, dn only with `pre`
+ *   dr           NULL: zero (then `pre`)
+ *   dx, dh       of the maps' type; dh NULL: no branch
+ *   dgate        SRHIP_GATE_ROWS: fp32 (rows / rows_per_gate, c);  SRHIP_GATE_MAP: of the gate's type
+ *   dscale       fp32 on the device, or NULL
+ *   d*_bias      fp32[c] or NULL
+ *   workspace    srhip_norm_residual_bwd_workspace_bytes(args) bytes (a function of rows, rows_per_gate, c and gate_mode)
+ * rows >= 1.  Deterministic: sums over rows are added in a fixed order, without atomics. */
+typedef struct {
+    const void* h;
+    const void* h_scales;
+    const void* r;
+    const void* r_scales;
+    const void* dr;
+    const void* dn;
+    const void* gate;
+    const float* post_weight;
+    const float* post_bias;
+    const float* pre_weight;
+    const float* scale_ptr;
+    void* dx;
+    void* dh;
+    void* dgate;
+    float* dpost_weight;
+    float* dpost_bias;
+    float* dpre_weight;
+    float* dpre_bias;
+    float* dscale;
+    void* workspace;
+    long long rows, rows_per_gate;
+    int c, dtype, kind, post, pre, gate_mode, gate_f32, gate_sigmoid;
+    float scale, eps;
+} srhip_norm_residual_bwd_args;
+SRHIP_API size_t srhip_norm_residual_bwd_workspace_bytes(const srhip_norm_residual_bwd_args* args);
+SRHIP_API int srhip_norm_residual_bwd(const srhip_norm_residual_bwd_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -86,6 +86,21 @@ class Conv1x1ChainArgs(ctypes.Structure):
     ]
 
 
+class NormResidualArgs(ctypes.Structure):
+    """srhip_norm_residual_args"""
+    _fields_ = [(k, c_void_p) for k in ("x", "h", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias", "scale_ptr", "r", "n")] + [
+        ("rows", ctypes.c_longlong), ("rows_per_gate", ctypes.c_longlong)] + [
+        (k, c_int) for k in ("c", "dtype", "kind", "post", "pre", "gate_mode", "gate_f32", "gate_sigmoid")] + [("scale", c_float), ("eps", c_float)]
+
+
+class NormResidualBwdArgs(ctypes.Structure):
+    """srhip_norm_residual_bwd_args"""
+    _fields_ = [(k, c_void_p) for k in ("h", "h_scales", "r", "r_scales", "dr", "dn", "gate", "post_weight", "post_bias", "pre_weight", "scale_ptr",
+                                        "dx", "dh", "dgate", "dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias", "dscale", "workspace")] + [
+        ("rows", ctypes.c_longlong), ("rows_per_gate", ctypes.c_longlong)] + [
+        (k, c_int) for k in ("c", "dtype", "kind", "post", "pre", "gate_mode", "gate_f32", "gate_sigmoid")] + [("scale", c_float), ("eps", c_float)]
+
+
 _SIGNATURES = {
     "srhip_version": (c_int, []),
     "srhip_last_error": (ctypes.c_char_p, []),
@@ -109,6 +124,14 @@ _SIGNATURES = {
     "srhip_conv3x3_wgrad_windows": (c_int, [c_void_p] * 5 + [c_int] * 10 + [c_float] + [c_int] * 4 + [c_void_p]),
     "srhip_conv3x3_wgrad_multi": (c_int, [ctypes.POINTER(WgradJob), c_int, c_void_p] + [c_int] * 7 + [c_float, c_void_p]),
     "srhip_conv1x1_wgrad_multi": (c_int, [ctypes.POINTER(WgradJob), c_int, c_void_p] + [c_int] * 7 + [c_float, c_void_p]),
+    "srhip_conv_wgrad_checkpoint8": (c_int, [ctypes.POINTER(WgradJob), ctypes.POINTER(c_void_p), c_int, c_void_p] + [c_int] * 8 + [c_float, c_void_p]),
+    "srhip_checkpoint8_pack": (c_int, [c_void_p, c_int, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_void_p]),
+    "srhip_checkpoint8_pack_signbits": (c_int, [c_void_p] * 4 + [c_int] * 3 + [c_void_p]),
+    "srhip_checkpoint8_restore": (c_int, [c_void_p, c_void_p, c_void_p, c_int, ctypes.c_longlong, c_int, c_void_p]),
+    "srhip_relu_mask_checkpoint8": (c_int, [c_void_p] * 3 + [c_size_t, c_void_p]),
+    "srhip_norm_residual_fwd": (c_int, [ctypes.POINTER(NormResidualArgs), c_void_p]),
+    "srhip_norm_residual_bwd_workspace_bytes": (c_size_t, [ctypes.POINTER(NormResidualBwdArgs)]),
+    "srhip_norm_residual_bwd": (c_int, [ctypes.POINTER(NormResidualBwdArgs), c_void_p]),
     "srhip_conv2d_direct": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p] + [c_int] * 13 +
                             [c_int, c_float, c_float, c_void_p]),
     "srhip_upsample_grid_bilinear_nhwc": (c_int, [c_void_p, c_void_p] + [c_int] * 6 + [c_void_p]),

@@ -242,11 +242,6 @@ def nhwc_to_nchw_f32(x: Tensor, c: int) -> Tensor:
 # Any layer functional.conv2d_auto runs (kernel 1 or 3, stride 1 or 2, any channel counts, up to three concatenated
 # sources), differentiable: the temporal network's training graph (core/models/model_final.py under loss.backward()).
 # ------------------------------------------------------------------------------------------------
-def _tile_channels(c: int) -> int:
-    """Channel count of a slice as the weight-gradient kernel tiles it (16, 32 or 64)."""
-    return 16 if c <= 16 else (32 if c <= 32 else 64)
-
-
 def _zero_insert2(dz: Tensor, h: int, w: int) -> Tensor:
     """(N,ho,wo,C) -> (N,h,w,C) with dz at the even positions: a stride-2 layer's output gradient seen from the
     stride-1 layer it is a 2x2 pick of (its data and weight gradients are that layer's on this tensor)."""
@@ -298,37 +293,10 @@ class _ConvAuto(Function):
 
 def _auto_wgrad(srcs, dzs: Tensor, w: Tensor):
     """Weight and bias gradient of a layer of ``_ConvAuto`` from the gradient of its (equivalent stride-1) pre-activation:
-    the MFMA weight-gradient kernel per (<= 64 input, <= 64 output) channel slice pair; a 1x1 layer is the centre tap of
-    the 3x3 result (a GEMM over a million pixels with a 160 x 160 output is a shape the GEMM library serves three times
-    slower than that).  The kernel reads the channel windows in place: no slice of x or dz is copied out."""
+    the MFMA weight-gradient kernel per (<= 64 input, <= 64 output) channel slice pair (a GEMM over a million pixels with a
+    160 x 160 output is a shape the GEMM library serves three times slower than that)."""
     cout, cin, k, _ = w.shape
-    # (every entry is written: the slice pairs tile the whole weight, the first input slice's jobs the whole bias)
-    # (a 1x1 layer: the kernel's centre-tap form writes the (O,I,1,1) gradient directly; SRHIP_NO_WGRAD_1X1=1: as the centre
-    # tap of the 3x3 result, eight taps computed and dropped)
-    k_out = 1 if (k == 1 and os.environ.get("SRHIP_NO_WGRAD_1X1", "0") != "1") else 3
-    dw3 = torch.empty((cout, cin, k_out, k_out), dtype=torch.float32, device=w.device)
-    db = torch.empty((cout,), dtype=torch.float32, device=w.device)
-    dz_slices = [(o, min(64, cout - o)) for o in range(0, cout, 64)]
-    # all slice pairs of one tile shape go out together (one gradient launch + one reduction per group of <= 32 pairs
-    # instead of one each per pair: on the 1/4 and 1/8 resolution maps a pair is a few microseconds of matrix work)
-    groups = {}
-    k0 = 0
-    for t in srcs:
-        for a in range(0, t.shape[-1], 64):
-            ci = min(a + 64, t.shape[-1]) - a
-            ci_real = min(ci, cin - (k0 + a))
-            if ci_real <= 0:
-                continue
-            for o, co in dz_slices:
-                # the bias gradient rides on the first input slice's job (dz times ones on the MFMA pipe)
-                groups.setdefault((_tile_channels(ci), _tile_channels(co)), []).append(
-                    (t, a, ci_real, k0 + a, dzs, o, co, o, k0 + a == 0))
-        k0 += t.shape[-1]
-    batch = 1 if os.environ.get("SRHIP_NO_WGRAD_MULTI", "0") == "1" else F_.WGRAD_MAX_JOBS
-    for (ci_tile, co_tile), jobs in groups.items():
-        for b in range(0, len(jobs), batch):
-            F_.conv3x3_wgrad_multi(jobs[b:b + batch], dw3, db, ci_tile, co_tile)
-    return (dw3 if k == k_out else dw3[:, :, 1:2, 1:2].contiguous()), db
+    return F_.conv_wgrad(srcs, dzs, cin, cout, k)
 
 
 def _dgrad_rows(dzs: Tensor, w: Tensor, row0: int, rows: int, mask: Tensor = None) -> Tensor:

@@ -20,12 +20,18 @@
 //   * Accumulators persist over every work item of the workgroup; at the end each wave writes its
 //     partial tiles to the workspace and a second kernel sums them in a fixed order
 //     (deterministic, no atomics) into the fp32 OIHW gradient.
+//   * X8 form: xin is an 8-bit checkpoint (checkpoint8.hip), e4m3 codes with a scale byte per 32 channels.  Its rows travel
+//     HBM -> registers three rows ahead (16 codes and their scale byte to a lane and piece), are decoded to bf16 -- exactly,
+//     the scales are powers of two -- once per element, and written to a two-slot LDS ring one row before they are read;
+//     from there on the loop is the same, and so are its results on the restored map, bit for bit.  Decoding what the
+//     matrix unit reads instead would repeat it for every wave and tap column.
 //   * LDS image [pixel][channel]; for 64-channel rows the two 64-byte halves of a pixel are swapped
 //     on every second pixel pair (applied on the SOURCE side of the DMA) so that the transposing
 //     reads of 4 consecutive pixels x 32 channels touch every bank once.
 #include <atomic>
+#include <type_traits>
 
-#include "srhip_common.h"
+#include "rows_util.h"
 #define SRHIP_CAPTURE(x) (void)&(x)   // asm operands alone do not make a generic lambda capture
 
 namespace {
@@ -48,6 +54,11 @@ struct WgradParams {
     int njobs, wgs_per_job;
     WgradJob jobs[kMaxJobs];
 };
+// the X8 form's x: codes in WgradJob::x (xs, xco in bytes = channels), scale bytes beside them
+struct WgradParams8 : WgradParams {
+    const char* xscale[kMaxJobs];
+    int xsb[kMaxJobs];   // scale bytes per pixel
+};
 struct WgradOut {
     float* dw;   // first output row of the job's co slice
     float* db;   // or null
@@ -69,9 +80,11 @@ constexpr unsigned kOob = 0x80000000u;
 // TAPS = 9: the 3x3 layer.  TAPS = 1: a 1x1 layer (core/models/model_final.py:237-246) = the centre tap alone -- one
 // accumulator tile instead of nine, 8 MFMAs per row and wave instead of 72 (as the centre tap of the full kernel a 1x1
 // layer paid for eight taps it threw away).
-template <int CI_, int CO_, int TAPS_ = 9>
+template <int CI_, int CO_, int TAPS_ = 9, bool X8_ = false>
 struct WCfg {
     static constexpr int CI = CI_, CO = CO_, TAPS = TAPS_;
+    static constexpr bool X8 = X8_;
+    using Params = std::conditional_t<X8, WgradParams8, WgradParams>;
     static constexpr int KX0 = TAPS == 9 ? 0 : 1, KX1 = TAPS == 9 ? 3 : 2;   // tap columns walked
     static_assert(TAPS == 9 || TAPS == 1, "3x3 or its centre tap");
     static constexpr int NWAVES = 4, TW = 128;
@@ -87,15 +100,18 @@ struct WCfg {
     static constexpr int ZNP = TW / ZPP;
     static constexpr int X_SLOT = XNP * 1024, Z_SLOT = ZNP * 1024;
     static constexpr int XA = 3, ZA = 3;          // rows issued ahead
-    static constexpr int XRING = XA + 1, ZRING = ZA + 1;
+    static constexpr int XRING = X8 ? 2 : XA + 1, ZRING = ZA + 1;
     static constexpr int Z_BASE = XRING * X_SLOT;
     static constexpr int SINK_OFF = Z_BASE + ZRING * Z_SLOT;     // 1 KiB sink of the DMA pieces a wave does not own
     static constexpr int LDS_BYTES = SINK_OFF + 1024;
-    static constexpr int MAXPX = (XNP + NWAVES - 1) / NWAVES, MINPX = XNP / NWAVES;
+    static constexpr int MAXPX = X8 ? 0 : (XNP + NWAVES - 1) / NWAVES, MINPX = X8 ? 0 : XNP / NWAVES;
+    // X8: 16-code chunks of a row (halo included), and how many a lane takes
+    static constexpr int CPP8 = CI / 16, NCH8 = (TW + 2) * CPP8, MAXC8 = (NCH8 + NWAVES * 64 - 1) / (NWAVES * 64);
     static constexpr int MAXPZ = (ZNP + NWAVES - 1) / NWAVES, MINPZ = ZNP / NWAVES;
     // Every wave issues exactly MAXPX + MAXPZ pieces per iteration (a piece it does not own goes,
     // all-out-of-range, to the sink), x pieces first.  Top of iteration r needs x row r and dz row r,
-    // both issued in iteration r-XA: younger are exactly XA-1 whole iterations.
+    // both issued in iteration r-XA: younger are exactly XA-1 whole iterations.  (X8: the pieces are dz's alone; loads of
+    // codes that the compiler has placed between them only make the wait stricter.)
     static constexpr int TOP_WAIT = (XA - 1) * (MAXPX + MAXPZ);
     static_assert(XA == ZA && XA >= 2, "wait counts assume both rings run the same distance ahead");
     static_assert(LDS_BYTES <= 160 * 1024, "rings exceed the CU's LDS");
@@ -162,8 +178,22 @@ __device__ __forceinline__ unsigned img_off(int px, int cb)
     return (unsigned)(px * PB + cb);
 }
 
+// X8: decodes a lane's 16 codes and writes the 32 bytes to the LDS image
+__device__ __forceinline__ void decode_to_lds(const rows_u32x4 q, const float scale, const unsigned addr)
+{
+    rows_u32x4 lo, hi;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float f[4];
+        ck8_unpack4(q[j], scale, f);
+        (j < 2 ? lo : hi)[2 * (j & 1)] = pack_bf16x2(f[0], f[1]);
+        (j < 2 ? lo : hi)[2 * (j & 1) + 1] = pack_bf16x2(f[2], f[3]);
+    }
+    asm volatile("ds_write_b128 %0, %1\n\tds_write_b128 %0, %2 offset:16" ::"v"(addr), "v"(lo), "v"(hi) : "memory");
+}
+
 template <class C>
-__global__ __launch_bounds__(C::NWAVES * 64, 1) void conv3x3_wgrad_kernel(const WgradParams p)
+__global__ __launch_bounds__(C::NWAVES * 64, 1) void conv3x3_wgrad_kernel(const typename C::Params p)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x;
@@ -224,8 +254,42 @@ __global__ __launch_bounds__(C::NWAVES * 64, 1) void conv3x3_wgrad_kernel(const 
         const __amdgpu_buffer_rsrc_t rsrc_z =
             __builtin_amdgcn_make_buffer_rsrc((void*)(jb.dz + (long long)n * img_z), 0, (int)img_z, 0x00020000);
 
+        // X8: a lane's chunks of a row, in HBM (codes, scale byte) and in the LDS image; three rows of them in registers,
+        // register set = row % 3
+        __amdgpu_buffer_rsrc_t rsrc_s = rsrc_x;
+        rows_u32x4 code[3][C::MAXC8];
+        unsigned sbyte[3][C::MAXC8], coff[C::MAXC8], soff[C::MAXC8], laddr[C::MAXC8];
+        unsigned xsb = 0;   // scale bytes per pixel
+        if constexpr (C::X8) {
+            xsb = (unsigned)p.xsb[job];
+            const unsigned img_s = (unsigned)(H * W) * xsb;
+            rsrc_s = __builtin_amdgcn_make_buffer_rsrc((void*)(p.xscale[job] + (long long)n * img_s), 0, (int)img_s, 0x00020000);
+#pragma unroll
+            for (int m = 0; m < C::MAXC8; ++m) {
+                const int L = tid + m * C::NWAVES * 64, px = L / C::CPP8, s = L % C::CPP8, col = x0 - 1 + px;
+                const bool ok = col >= 0 && col < W && px < C::TW + 2;
+                coff[m] = ok ? (unsigned)(col * jb.xs + jb.xco + s * 16) : kOob;
+                soff[m] = ok ? (unsigned)col * xsb + (unsigned)((jb.xco + s * 16) / kCk8Group) : kOob;
+                laddr[m] = lds_base + img_off<C::XPB>(px, s * 32);
+            }
+        }
+        auto load_codes = [&](auto m_c, auto set_c, const int r) {   // x row r -> register set
+            SRHIP_CAPTURE(code); SRHIP_CAPTURE(sbyte); SRHIP_CAPTURE(coff); SRHIP_CAPTURE(soff);
+            constexpr int m = decltype(m_c)::value, set = decltype(set_c)::value;
+            const int y = y0 - 1 + r;
+            const bool in = (y >= 0) & (y < H) & (r < nout + 2);
+            code[set][m] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_x, coff[m], in ? (unsigned)(y * W) * (unsigned)jb.xs : kOob, 0);
+            sbyte[set][m] = __builtin_amdgcn_raw_buffer_load_b8(rsrc_s, soff[m], in ? (unsigned)(y * W) * xsb : kOob, 0);
+        };
+        auto write_codes = [&](auto m_c, auto set_c, const int slot) {   // register set -> LDS slot
+            SRHIP_CAPTURE(code); SRHIP_CAPTURE(sbyte); SRHIP_CAPTURE(laddr);
+            constexpr int m = decltype(m_c)::value, set = decltype(set_c)::value;
+            if (tid + m * C::NWAVES * 64 < C::NCH8)
+                decode_to_lds(code[set][m], ck8_scale(sbyte[set][m]), laddr[m] + (unsigned)(slot * C::X_SLOT));
+        };
+
         // per-lane source offsets of this wave's DMA pieces (constant over the strip)
-        unsigned xoff[C::MAXPX], zoff[C::MAXPZ];
+        unsigned xoff[C::MAXPX > 0 ? C::MAXPX : 1], zoff[C::MAXPZ];
 #pragma unroll
         for (int m = 0; m < C::MAXPX; ++m) {
             const int L = (wave + m * C::NWAVES) * 64 + lane;  // 16-B chunk index inside the row slot
@@ -268,10 +332,16 @@ __global__ __launch_bounds__(C::NWAVES * 64, 1) void conv3x3_wgrad_kernel(const 
         };
 
         __builtin_amdgcn_s_barrier();  // every wave is done reading the previous item's rows
+        if constexpr (C::X8) {   // row 0 -> LDS, rows 1 .. 3 -> register sets 1, 2, 0
+            wg_static_for<0, C::MAXC8>([&](auto m_c) { load_codes(m_c, WIntC<0>{}, 0); load_codes(m_c, WIntC<1>{}, 1); load_codes(m_c, WIntC<2>{}, 2); });
+            wg_static_for<0, C::MAXC8>([&](auto m_c) { write_codes(m_c, WIntC<0>{}, 0); load_codes(m_c, WIntC<0>{}, 3); });
+            wg_lds_wait<0>();   // before the barrier in front of row 0
+        } else {
 #pragma unroll 1
-        for (int r = 0; r < C::XA; ++r) {
-            const unsigned so = x_soff(r);
-            wg_static_for<0, C::MAXPX>([&](auto m_c) { issue_piece(m_c, so, (unsigned)(r * C::X_SLOT), 0u, 0u); });
+            for (int r = 0; r < C::XA; ++r) {
+                const unsigned so = x_soff(r);
+                wg_static_for<0, C::MAXPX>([&](auto m_c) { issue_piece(m_c, so, (unsigned)(r * C::X_SLOT), 0u, 0u); });
+            }
         }
 #pragma unroll 1
         for (int r = 0; r < C::ZA; ++r) {
@@ -291,7 +361,7 @@ __global__ __launch_bounds__(C::NWAVES * 64, 1) void conv3x3_wgrad_kernel(const 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { alo[j][k][e] = 0; ahi[j][k][e] = 0; }
 
-        int ring = 0;   // ring slot of x row r and of dz row r (both rings have XRING slots)
+        int ring = 0;   // ring slot of x row r and of dz row r (both rings have XRING slots; X8: of dz row r alone)
         auto row_body = [&](auto ph_c, const int r) {
             SRHIP_CAPTURE(alo); SRHIP_CAPTURE(ahi); SRHIP_CAPTURE(acc); SRHIP_CAPTURE(accb);
             constexpr int PH = decltype(ph_c)::value;   // r % 3: register slot of dz row r
@@ -300,6 +370,7 @@ __global__ __launch_bounds__(C::NWAVES * 64, 1) void conv3x3_wgrad_kernel(const 
             __builtin_amdgcn_s_barrier();
             // rows fetched during this iteration go to the slots that row r-1 just left
             const unsigned dxs = x_soff(r + C::XA), dzs = z_soff(r + C::ZA);
+            const int xslot = C::X8 ? r & 1 : ring;
             const unsigned dxslot = (unsigned)((ring == 0 ? C::XRING - 1 : ring - 1) * C::X_SLOT);
             const unsigned dzslot = (unsigned)(C::Z_BASE + (ring == 0 ? C::ZRING - 1 : ring - 1) * C::Z_SLOT);
             // per-row read bases: everything else is an immediate offset of the LDS instruction
@@ -308,9 +379,9 @@ __global__ __launch_bounds__(C::NWAVES * 64, 1) void conv3x3_wgrad_kernel(const 
             for (int j2 = 0; j2 < 2; ++j2) {
                 za[j2] = zaddr[j2] + (unsigned)(ring * C::Z_SLOT);
 #pragma unroll
-                for (int kx = 0; kx < 3; ++kx) xa[kx][j2] = xaddr[kx][j2] + (unsigned)(ring * C::X_SLOT);
+                for (int kx = 0; kx < 3; ++kx) xa[kx][j2] = xaddr[kx][j2] + (unsigned)(xslot * C::X_SLOT);
             }
-            ring = (ring + 1 == C::XRING) ? 0 : ring + 1;
+            ring = (ring + 1 == C::ZRING) ? 0 : ring + 1;
 
             // dz fragments of row r -> register slot PH
             wg_static_for<0, C::NKS>([&](auto s_c) {
@@ -362,6 +433,15 @@ __global__ __launch_bounds__(C::NWAVES * 64, 1) void conv3x3_wgrad_kernel(const 
                     // bias gradient: the waves that share an output-channel tile take turns over the k-steps, so that
                     // every wave issues the same number of MFMAs per row (the reduction adds their partial sums)
                     if (cit == sk % C::CIT) wg_mfma<9>(accb, join(alo[PH][sk], ahi[PH][sk]), ones);
+                }
+                // X8: row r + 1 from registers to LDS, its registers to row r + 4, spread over the first steps and never in
+                // the last, whose wait covers the writes (the counted waits in between get stricter by them, not weaker)
+                if constexpr (C::X8) {
+                    constexpr int CPS = (C::MAXC8 + (NSTEP - ST0) - 2) / (NSTEP - ST0 - 1);
+                    wg_static_for<((st - ST0) * CPS < C::MAXC8 ? (st - ST0) * CPS : C::MAXC8), ((st - ST0 + 1) * CPS < C::MAXC8 ? (st - ST0 + 1) * CPS : C::MAXC8)>([&](auto m_c) {
+                        write_codes(m_c, WIntC<(PH + 1) % 3>{}, (r + 1) & 1);
+                        load_codes(m_c, WIntC<(PH + 1) % 3>{}, r + 4);
+                    });
                 }
                 // the LDS-DMA pieces of the rows two iterations ahead, spread over the first steps
                 wg_static_for<(st - ST0) * PPS, ((st - ST0 + 1) * PPS < NP ? (st - ST0 + 1) * PPS : NP)>([&](auto m_c) {
@@ -475,7 +555,7 @@ __global__ __launch_bounds__(1024) void wgrad_reduce_kernel(const ReduceParams r
 }
 
 template <class C>
-int launch_wgrad(WgradParams p, const WgradOut* outs, int w_i, int accumulate, float scale, hipStream_t stream)
+int launch_wgrad(typename C::Params p, const WgradOut* outs, int w_i, int accumulate, float scale, hipStream_t stream)
 {
     static std::atomic<bool> configured_dev[kSrhipMaxDevices];   // per device
     const int dev = srhip_current_device();
@@ -548,13 +628,14 @@ SRHIP_API size_t srhip_conv3x3_wgrad_workspace_bytes(void)
     return (size_t)srhip_num_cus() * 4 * 10 * 1024 * sizeof(float);
 }
 
-static int wgrad_multi(const srhip_wgrad_job* jobs, int njobs, void* workspace, int n, int h, int w, int ci_pad, int co_pad,
+// x8: null, or (per job) the scale bytes of x, whose codes jobs[j].x then holds
+static int wgrad_multi(const srhip_wgrad_job* jobs, const void* const* x8, int njobs, void* workspace, int n, int h, int w, int ci_pad, int co_pad,
                        int w_i, int accumulate, float scale, int taps, void* stream)
 {
     SRHIP_REQUIRE(jobs && workspace, "conv3x3_wgrad: null pointer");
     SRHIP_REQUIRE(njobs >= 1 && njobs <= kMaxJobs, "conv3x3_wgrad: %d jobs (1 .. %d per call)", njobs, kMaxJobs);
     SRHIP_REQUIRE(n >= 1 && h >= 1 && w >= 1, "conv3x3_wgrad: empty tensor");
-    WgradParams p;
+    WgradParams8 p;
     WgradOut outs[kMaxJobs];
     p.partial = (float*)workspace;
     p.n = n; p.h = h; p.w = w;
@@ -570,12 +651,22 @@ static int wgrad_multi(const srhip_wgrad_job* jobs, int njobs, void* workspace, 
                       "conv3x3_wgrad: dz window [%d,%d) outside the map's %d channels (offsets and widths in multiples of 8)", a.dz_coff, a.dz_coff + a.co_real, a.dz_cstride);
         SRHIP_REQUIRE((long long)h * w * (a.x_cstride > a.dz_cstride ? a.x_cstride : a.dz_cstride) * 2 < (1ll << 31), "conv3x3_wgrad: image too large for 32-bit offsets");
         p.jobs[j].x = (const char*)a.x; p.jobs[j].dz = (const char*)a.dz;
-        p.jobs[j].xs = a.x_cstride * 2; p.jobs[j].xco = a.x_coff * 2; p.jobs[j].zs = a.dz_cstride * 2; p.jobs[j].zco = a.dz_coff * 2;
+        if (x8) {
+            SRHIP_REQUIRE(x8[j], "conv_wgrad_checkpoint8: null scales (job %d)", j);
+            SRHIP_REQUIRE(a.x_cstride % 16 == 0 && a.x_coff % 16 == 0 && ((size_t)a.x & 15) == 0, "conv_wgrad_checkpoint8: codes start at, and lie and are cut in, multiples of 16 channels (job %d)", j);
+        }
+        const int xsize = x8 ? 1 : 2;
+        p.xscale[j] = x8 ? (const char*)x8[j] : nullptr;
+        p.xsb[j] = srhip_div_up(a.x_cstride, kCk8Group);
+        p.jobs[j].xs = a.x_cstride * xsize; p.jobs[j].xco = a.x_coff * xsize; p.jobs[j].zs = a.dz_cstride * 2; p.jobs[j].zco = a.dz_coff * 2;
         outs[j].dw = a.dw; outs[j].db = a.db; outs[j].ci_off = a.ci_off; outs[j].ci_real = a.ci_real; outs[j].co_real = a.co_real; outs[j].pad = 0;
     }
-    for (int j = njobs; j < kMaxJobs; ++j) { p.jobs[j] = p.jobs[0]; }
+    for (int j = njobs; j < kMaxJobs; ++j) { p.jobs[j] = p.jobs[0]; p.xscale[j] = p.xscale[0]; p.xsb[j] = p.xsb[0]; }
     hipStream_t s = (hipStream_t)stream;
 #define SRHIP_WGRAD_CASE(CI, CO) \
+    if (ci_pad == CI && co_pad == CO && x8) \
+        return taps == 9 ? launch_wgrad<WCfg<CI, CO, 9, true>>(p, outs, w_i, accumulate, scale, s) \
+                         : launch_wgrad<WCfg<CI, CO, 1, true>>(p, outs, w_i, accumulate, scale, s); \
     if (ci_pad == CI && co_pad == CO) \
         return taps == 9 ? launch_wgrad<WCfg<CI, CO, 9>>(p, outs, w_i, accumulate, scale, s) \
                          : launch_wgrad<WCfg<CI, CO, 1>>(p, outs, w_i, accumulate, scale, s);
@@ -596,13 +687,21 @@ static int wgrad_multi(const srhip_wgrad_job* jobs, int njobs, void* workspace, 
 SRHIP_API int srhip_conv3x3_wgrad_multi(const srhip_wgrad_job* jobs, int njobs, void* workspace, int n, int h, int w,
                                         int ci_pad, int co_pad, int w_i, int accumulate, float scale, void* stream)
 {
-    return wgrad_multi(jobs, njobs, workspace, n, h, w, ci_pad, co_pad, w_i, accumulate, scale, 9, stream);
+    return wgrad_multi(jobs, nullptr, njobs, workspace, n, h, w, ci_pad, co_pad, w_i, accumulate, scale, 9, stream);
 }
 
 SRHIP_API int srhip_conv1x1_wgrad_multi(const srhip_wgrad_job* jobs, int njobs, void* workspace, int n, int h, int w,
                                         int ci_pad, int co_pad, int w_i, int accumulate, float scale, void* stream)
 {
-    return wgrad_multi(jobs, njobs, workspace, n, h, w, ci_pad, co_pad, w_i, accumulate, scale, 1, stream);
+    return wgrad_multi(jobs, nullptr, njobs, workspace, n, h, w, ci_pad, co_pad, w_i, accumulate, scale, 1, stream);
+}
+
+SRHIP_API int srhip_conv_wgrad_checkpoint8(const srhip_wgrad_job* jobs, const void* const* x_scales, int njobs, void* workspace, int n, int h, int w,
+                                           int ci_pad, int co_pad, int w_i, int ksize, int accumulate, float scale, void* stream)
+{
+    SRHIP_REQUIRE(x_scales, "conv_wgrad_checkpoint8: null pointer");
+    SRHIP_REQUIRE(ksize == 1 || ksize == 3, "conv_wgrad_checkpoint8: kernel size %d (1 or 3)", ksize);
+    return wgrad_multi(jobs, x_scales, njobs, workspace, n, h, w, ci_pad, co_pad, w_i, accumulate, scale, ksize * ksize, stream);
 }
 
 SRHIP_API int srhip_conv3x3_wgrad_windows(const void* x, const void* dz, float* dw, float* db, void* workspace, int n, int h,

@@ -1,0 +1,174 @@
+// The norms around a residual block, with its gate and residual scale, in one pass over the rows of a channels-last map:
+//
+//   p = N_post(h) = (h - mean h) / sqrt(var h + eps) * w + b          (layer; rms: h / sqrt(mean h^2 + eps) * w; none: h)
+//   r = x + s * act(g) * p                                            (the residual sum: what the next block adds to)
+//   n = N_pre(r)                                                      (what the next block reads)
+//
+// Layer by layer this is LayerNorm (core/arch/CAMixerSR.py:29-37), a gated map (core/arch/RepRFN.py:233-235), a scaled
+// residual sum (core/models/model.py:33) and LayerNorm again: ten passes over maps of which four or five are left.
+// n is the norm of the unrounded sum.  All arithmetic in fp32, each output rounded once.
+//
+// Bound by HBM: x, h (and a gate map) are read once, r and n written once, a row stays in the registers of its lanes.
+#include "norm_residual.h"
+
+namespace {
+
+struct NormParams {
+    const char* x;
+    const char* h;
+    const char* gate;
+    const float *post_w, *post_b, *pre_w, *pre_b, *scale_ptr;
+    char* r;
+    char* n;
+    long long rows, rows_per_gate;
+    int c, layer, post, pre, gate_mode, gate_f32, sigmoid;
+    float scale, eps, inv_c;
+};
+
+template <class C>
+__global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormParams p)
+{
+    using T = typename C::T;
+    constexpr int SIZE = RowVec<T>::SIZE, VEC = C::VEC;
+    __shared__ float scratch[row_sum_scratch<C>()];
+    RowSum<C> sum{scratch, 0};
+    const int t = threadIdx.x % C::TPR, rg = threadIdx.x / C::TPR;
+    int c0[C::V], nv[C::V];
+    float wpost[C::E], bpost[C::E], wpre[C::E], bpre[C::E], g[C::E];
+#pragma unroll
+    for (int v = 0; v < C::V; ++v) {
+        c0[v] = (v * C::TPR + t) * VEC;
+        nv[v] = p.c - c0[v];
+        load_params<C>(p.post_w, c0[v], nv[v], 1.0f, wpost + v * VEC);
+        load_params<C>(p.post_b, c0[v], nv[v], 0.0f, bpost + v * VEC);
+        load_params<C>(p.pre_w, c0[v], nv[v], 1.0f, wpre + v * VEC);
+        load_params<C>(p.pre_b, c0[v], nv[v], 0.0f, bpre + v * VEC);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) g[v * VEC + j] = 1.0f;
+    }
+    const float scale = p.scale_ptr ? *p.scale_ptr : p.scale;
+    long long gate_end = 0;   // first row that the gate held in registers does not belong to
+
+    for (long long base = (long long)blockIdx.x * C::RPB; base < p.rows; base += (long long)gridDim.x * C::RPB) {
+        const bool live = base + rg < p.rows;
+        const long long row = live ? base + rg : p.rows - 1;   // lanes behind the last row work on it too and store nothing
+        const long long at = row * p.c;
+        rows_u32x4 qx[C::V], qh[C::V], qg[C::V];
+#pragma unroll
+        for (int v = 0; v < C::V; ++v) qx[v] = load_row16<T>(p.x + (at + c0[v]) * SIZE, nv[v]);
+        if (p.h)
+#pragma unroll
+            for (int v = 0; v < C::V; ++v) qh[v] = load_row16<T>(p.h + (at + c0[v]) * SIZE, nv[v]);
+        if (p.gate_mode == SRHIP_GATE_MAP) {
+            if (p.gate_f32) {
+#pragma unroll
+                for (int v = 0; v < C::V; ++v) load_params<C>((const float*)p.gate + at, c0[v], nv[v], 0.0f, g + v * VEC);
+            } else {
+#pragma unroll
+                for (int v = 0; v < C::V; ++v) qg[v] = load_row16<T>(p.gate + (at + c0[v]) * SIZE, nv[v]);
+#pragma unroll
+                for (int v = 0; v < C::V; ++v) RowVec<T>::unpack(qg[v], g + v * VEC);
+            }
+        } else if (p.gate_mode == SRHIP_GATE_ROWS && row >= gate_end) {   // rows of a lane only grow
+            const long long s = row / p.rows_per_gate;
+            gate_end = (s + 1) * p.rows_per_gate;
+#pragma unroll
+            for (int v = 0; v < C::V; ++v) load_params<C>((const float*)p.gate + s * p.c, c0[v], nv[v], 0.0f, g + v * VEC);
+            if (p.sigmoid)
+#pragma unroll
+                for (int j = 0; j < C::E; ++j) g[j] = sigmoid_f32(g[j]);
+        }
+        if (p.gate_mode == SRHIP_GATE_MAP && p.sigmoid)
+#pragma unroll
+            for (int j = 0; j < C::E; ++j) g[j] = sigmoid_f32(g[j]);
+
+        float r[C::E];
+#pragma unroll
+        for (int v = 0; v < C::V; ++v) RowVec<T>::unpack(qx[v], r + v * VEC);
+        if (p.h) {
+            float h[C::E];
+#pragma unroll
+            for (int v = 0; v < C::V; ++v) RowVec<T>::unpack(qh[v], h + v * VEC);
+            if (p.post) {
+                float mean, rstd;
+                row_statistics<C>(sum, h, nv, p.layer, p.inv_c, p.eps, mean, rstd);
+#pragma unroll
+                for (int j = 0; j < C::E; ++j) h[j] = (h[j] - mean) * rstd * wpost[j] + bpost[j];
+            }
+#pragma unroll
+            for (int v = 0; v < C::V; ++v) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    const int j = v * VEC + k;
+                    r[j] = k < nv[v] ? r[j] + scale * (g[j] * h[j]) : 0.0f;
+                }
+                if (live) store_row16<T>(p.r + (at + c0[v]) * SIZE, RowVec<T>::pack(r + v * VEC), nv[v]);
+            }
+        }
+        if (p.pre) {
+            float mean, rstd;
+            row_statistics<C>(sum, r, nv, p.layer, p.inv_c, p.eps, mean, rstd);
+#pragma unroll
+            for (int j = 0; j < C::E; ++j) r[j] = (r[j] - mean) * rstd * wpre[j] + bpre[j];
+            if (live)
+#pragma unroll
+                for (int v = 0; v < C::V; ++v) store_row16<T>(p.n + (at + c0[v]) * SIZE, RowVec<T>::pack(r + v * VEC), nv[v]);
+        }
+    }
+}
+
+template <class C>
+int launch(const NormParams& p, hipStream_t stream)
+{
+    // as many work-groups as are resident at once: each keeps its parameters in registers over all its rows
+    const long long want = (p.rows + C::RPB - 1) / C::RPB;
+    const long long resident = (long long)srhip_num_cus() * (2048 / C::THREADS);
+    hipLaunchKernelGGL(norm_residual_kernel<C>, dim3((unsigned)(want < resident ? want : resident)), dim3(C::THREADS), 0, stream, p);
+    return srhip_check_launch("norm_residual_kernel");
+}
+
+// the narrowest group of lanes that holds a row
+template <class T>
+int dispatch(const NormParams& p, hipStream_t s)
+{
+    constexpr int K = 8 / RowVec<T>::VEC;   // vectors for 8 channels
+    if (p.c <= 16) return launch<RowCfg<T, 2, K>>(p, s);
+    if (p.c <= 32) return launch<RowCfg<T, 4, K>>(p, s);
+    if (p.c <= 64) return launch<RowCfg<T, 8, K>>(p, s);
+    if (p.c <= 128) return launch<RowCfg<T, 16, K>>(p, s);
+    if (p.c <= 256) return launch<RowCfg<T, 32, K>>(p, s);
+    if (p.c <= 512) return launch<RowCfg<T, 64, K>>(p, s);
+    if (p.c <= 1024) return launch<RowCfg<T, 64, 2 * K>>(p, s);
+    if (p.c <= 2048) return launch<RowCfg<T, 256, K>>(p, s);
+    if (p.c <= 4096) return launch<RowCfg<T, 256, 2 * K>>(p, s);
+    return launch<RowCfg<T, 512, 2 * K>>(p, s);
+}
+
+}  // namespace
+
+extern "C" SRHIP_API int srhip_norm_residual_fwd(const srhip_norm_residual_args* a, void* stream)
+{
+    SRHIP_REQUIRE(a, "norm_residual: null pointer");
+    SRHIP_REQUIRE(a->rows >= 0 && a->c >= 1 && a->c <= SRHIP_NORM_MAX_C, "norm_residual: bad shape (%lld rows of %d channels; 1 .. %d channels)", a->rows, a->c, SRHIP_NORM_MAX_C);
+    SRHIP_REQUIRE(a->dtype == SRHIP_DT_BF16 || a->dtype == SRHIP_DT_F32, "norm_residual: unknown type %d", a->dtype);
+    SRHIP_REQUIRE(a->kind == SRHIP_NORM_LAYER || a->kind == SRHIP_NORM_RMS, "norm_residual: unknown norm %d", a->kind);
+    SRHIP_REQUIRE(a->gate_mode >= SRHIP_GATE_NONE && a->gate_mode <= SRHIP_GATE_MAP, "norm_residual: unknown gate mode %d", a->gate_mode);
+    SRHIP_REQUIRE(a->eps >= 0.0f, "norm_residual: eps must not be negative");
+    if (a->rows == 0) return SRHIP_OK;   // (pointers of empty maps may be null)
+    SRHIP_REQUIRE(a->h || a->pre, "norm_residual: neither a branch nor a norm behind the sum");
+    SRHIP_REQUIRE(a->h || (!a->post && a->gate_mode == SRHIP_GATE_NONE), "norm_residual: a gate or a post norm without a branch");
+    SRHIP_REQUIRE(a->x && (!a->h || a->r) && (!a->pre || (a->n && a->pre_weight)) && (!a->post || a->post_weight), "norm_residual: null pointer");
+    SRHIP_REQUIRE(a->gate_mode == SRHIP_GATE_NONE || a->gate, "norm_residual: null gate");
+    SRHIP_REQUIRE(a->gate_mode != SRHIP_GATE_ROWS || (a->rows_per_gate >= 1 && a->rows % a->rows_per_gate == 0), "norm_residual: %lld rows are not a multiple of %lld rows per gate", a->rows, a->rows_per_gate);
+    NormParams p;
+    p.x = (const char*)a->x; p.h = (const char*)a->h; p.gate = (const char*)a->gate;
+    p.post_w = a->post ? a->post_weight : nullptr; p.post_b = a->post ? a->post_bias : nullptr;
+    p.pre_w = a->pre ? a->pre_weight : nullptr; p.pre_b = a->pre ? a->pre_bias : nullptr;
+    p.scale_ptr = a->scale_ptr;
+    p.r = (char*)a->r; p.n = (char*)a->n;
+    p.rows = a->rows; p.rows_per_gate = a->rows_per_gate;
+    p.c = a->c; p.layer = a->kind == SRHIP_NORM_LAYER; p.post = a->post; p.pre = a->pre;
+    p.gate_mode = a->gate_mode; p.gate_f32 = a->dtype != SRHIP_DT_F32 && a->gate_f32; p.sigmoid = a->gate_sigmoid;
+    p.scale = a->scale; p.eps = a->eps; p.inv_c = 1.0f / (float)a->c;
+    return a->dtype == SRHIP_DT_BF16 ? dispatch<__bf16>(p, (hipStream_t)stream) : dispatch<float>(p, (hipStream_t)stream);
+}

@@ -4,14 +4,15 @@ Every function takes/returns torch tensors that live on a ROCm device; torch is 
 own device memory and to name the current HIP stream.  NHWC tensors are plain contiguous
 ``(N, H, W, C)`` bf16 tensors (not torch "channels_last" views).
 """
-from typing import Optional
+from typing import NamedTuple, Optional, Union
 
 import ctypes
 import os
 
 import torch
 
-from ._lib import Conv1x1ChainArgs, ConvGemmArgs, Conv3x3Args, Conv3x3PairArgs, check, lib
+from ._lib import (Conv1x1ChainArgs, ConvGemmArgs, Conv3x3Args, Conv3x3PairArgs, NormResidualArgs, NormResidualBwdArgs, WgradJob, check,
+                   lib)
 
 ACT_NONE, ACT_RELU, ACT_LRELU = 0, 1, 2
 RES_ADD, RES_MASK, RES_PRE = 0, 1, 2
@@ -284,7 +285,15 @@ def conv3x3_wgrad(x: torch.Tensor, dz: torch.Tensor, dw: torch.Tensor, db: Optio
     """dw[:, ci_off:ci_off+ci_real] (=|+=) weight gradient of a 3x3 layer from its input x (N,H,W,ci_pad) and the
     gradient dz (N,H,W,co_pad) of its pre-activation output; db (=|+=) bias gradient (or None).
     x_window / dz_window = (first_channel, tile) read channels [first_channel, first_channel + tile) of a wider map in
-    place (tile 16, 32 or 64; it may reach past the map's last channel, ci_real / co_real say how many channels count)."""
+    place (tile 16, 32 or 64; it may reach past the map's last channel, ci_real / co_real say how many channels count).
+    x may also be a checkpoint of the input (:class:`Checkpoint8`; windows at multiples of 16 channels)."""
+    if isinstance(x, Checkpoint8):
+        xo, xt = (0, x.shape[3]) if x_window is None else x_window
+        zo, zt = (0, dz.shape[3]) if dz_window is None else dz_window
+        if dw.dim() != 4 or tuple(dw.shape[2:]) != (3, 3):
+            raise ValueError("conv3x3_wgrad: dw must be a contiguous fp32 (O,I,3,3) tensor")
+        conv3x3_wgrad_multi([(x, xo, ci_real, ci_off, dz, zo, co_real, 0, db is not None)], dw, db, xt, zt, accumulate, scale)
+        return
     x = _req(x, torch.bfloat16, "x")
     dz = _req(dz, torch.bfloat16, "dz")
     if x.shape[:3] != dz.shape[:3]:
@@ -318,8 +327,8 @@ def conv3x3_wgrad_multi(jobs, dw: torch.Tensor, db: Optional[torch.Tensor], ci_t
     dw[co_off : co_off + co_real, ci_off : ci_off + ci_real] from channels [x_first_channel, + ci_tile) of the map x and
     [dz_first_channel, + co_tile) of the map dz (tiles 16, 32 or 64; a window may reach past its map's last channel), and,
     with_bias, db[co_off : co_off + co_real].  All maps share (N, H, W).  dw is the fp32 gradient of a (O,I,3,3) weight,
-    or of a (O,I,1,1) weight (srhip_conv1x1_wgrad_multi: the centre tap alone)."""
-    from ._lib import WgradJob
+    or of a (O,I,1,1) weight (srhip_conv1x1_wgrad_multi: the centre tap alone).
+    The x of the jobs may be checkpoints (:class:`Checkpoint8`, all of them or none; windows at multiples of 16 channels)."""
     if not 1 <= len(jobs) <= WGRAD_MAX_JOBS:
         raise ValueError("conv3x3_wgrad_multi: 1 .. %d jobs per call" % WGRAD_MAX_JOBS)
     if dw.dtype != torch.float32 or not dw.is_contiguous() or dw.dim() != 4 or tuple(dw.shape[2:]) not in ((3, 3), (1, 1)):
@@ -330,9 +339,21 @@ def conv3x3_wgrad_multi(jobs, dw: torch.Tensor, db: Optional[torch.Tensor], ci_t
     arr = (WgradJob * len(jobs))()
     shape = None
     w_i = dw.shape[1]
+    held = isinstance(jobs[0][0], Checkpoint8)
+    scales, alive = (ctypes.c_void_p * len(jobs))(), []
     for j, (x, xo, ci_real, ci_off, dz, zo, co_real, co_off, with_bias) in enumerate(jobs):
-        x = _req(x, torch.bfloat16, "x")
+        if isinstance(x, Checkpoint8) != held:
+            raise ValueError("conv3x3_wgrad_multi: maps and checkpoints in one call")
+        if held:
+            x, sc = _req_checkpoint8(x, "x")
+            scales[j] = sc.data_ptr()
+            alive.append(sc)
+            if x.dim() != 4:
+                raise ValueError("conv3x3_wgrad_multi: checkpoints of (N,H,W,C) maps")
+        else:
+            x = _req(x, torch.bfloat16, "x")
         dz = _req(dz, torch.bfloat16, "dz")
+        alive += [x, dz]   # contiguous copies live until the launch is queued
         if shape is None:
             shape = tuple(x.shape[:3])
         if tuple(x.shape[:3]) != shape or tuple(dz.shape[:3]) != shape:
@@ -346,14 +367,153 @@ def conv3x3_wgrad_multi(jobs, dw: torch.Tensor, db: Optional[torch.Tensor], ci_t
         a.ci_real, a.ci_off, a.co_real = ci_real, ci_off, co_real
         a.x_cstride, a.x_coff, a.dz_cstride, a.dz_coff, a.reserved = x.shape[3], xo, dz.shape[3], zo, 0
     n, h, w = shape
+    if held:
+        # a workspace of its own for every call: the allocator orders its reuse by stream and by captured graph
+        ws = torch.empty((lib.srhip_conv3x3_wgrad_workspace_bytes(),), dtype=torch.uint8, device=dw.device)
+        check(lib.srhip_conv_wgrad_checkpoint8(arr, scales, len(jobs), ws.data_ptr(), n, h, w, ci_tile, co_tile, w_i, dw.shape[2],
+                                               int(accumulate), scale, _stream()))
+        return
     entry = lib.srhip_conv3x3_wgrad_multi if taps == 9 else lib.srhip_conv1x1_wgrad_multi
     check(entry(arr, len(jobs), _wgrad_workspace(jobs[0][0].device).data_ptr(), n, h, w, ci_tile, co_tile, w_i, int(accumulate),
                 scale, _stream()))
 
 
-def relu_mask(dy: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """dy where y > 0 else 0 (bf16)."""
+def _tile_channels(c: int) -> int:
+    """Channel count of a slice as the weight-gradient kernel tiles it (16, 32 or 64)."""
+    return 16 if c <= 16 else (32 if c <= 32 else 64)
+
+
+def conv_wgrad(srcs, dz: torch.Tensor, cin: int, cout: int, ksize: int):
+    """Weight and bias gradient (dw (cout,cin,ksize,ksize), db (cout,), fp32) of a stride-1 layer with kernel 1 or 3 and any
+    channel counts, whose input is the concatenation of ``srcs`` (NHWC bf16 maps or their checkpoints), from the gradient dz
+    of its pre-activation output: one job per (<= 64 input, <= 64 output) channel slice pair, the channel windows read in
+    place.  SRHIP_NO_WGRAD_MULTI=1: a launch pair per job; SRHIP_NO_WGRAD_1X1=1: a 1x1 layer as the centre tap of a 3x3 one."""
+    if ksize not in (1, 3):
+        raise ValueError("conv_wgrad: kernel 1 or 3")
+    if cin < 1 or cout < 1 or cout > dz.shape[-1] or cin > sum(t.shape[-1] for t in srcs):
+        raise ValueError(f"conv_wgrad: {cin} -> {cout} channels of sources with {[t.shape[-1] for t in srcs]} and a gradient with {dz.shape[-1]}")
+    # (every entry is written: the slice pairs tile the whole weight, the first input slice's jobs the whole bias)
+    # (a 1x1 layer: the kernel's centre-tap form writes the (O,I,1,1) gradient directly)
+    k_out = 1 if (ksize == 1 and os.environ.get("SRHIP_NO_WGRAD_1X1", "0") != "1") else 3
+    dw = torch.empty((cout, cin, k_out, k_out), dtype=torch.float32, device=dz.device)
+    db = torch.empty((cout,), dtype=torch.float32, device=dz.device)
+    # all slice pairs of one tile shape go out together (one gradient launch + one reduction per group of <= 32 pairs
+    # instead of one each per pair: on the 1/4 and 1/8 resolution maps a pair is a few microseconds of matrix work)
+    groups = {}
+    k0 = 0
+    for t in srcs:
+        for a in range(0, t.shape[-1], 64):
+            ci = min(a + 64, t.shape[-1]) - a
+            ci_real = min(ci, cin - (k0 + a))
+            if ci_real <= 0:
+                continue
+            for o in range(0, cout, 64):
+                co = min(64, cout - o)
+                # the bias gradient rides on the first input slice's job (dz times ones on the MFMA pipe)
+                groups.setdefault((isinstance(t, Checkpoint8), _tile_channels(ci), _tile_channels(co)), []).append(
+                    (t, a, ci_real, k0 + a, dz, o, co, o, k0 + a == 0))
+        k0 += t.shape[-1]
+    batch = 1 if os.environ.get("SRHIP_NO_WGRAD_MULTI", "0") == "1" else WGRAD_MAX_JOBS
+    for (_, ci_tile, co_tile), jobs in groups.items():
+        for b in range(0, len(jobs), batch):
+            conv3x3_wgrad_multi(jobs[b:b + batch], dw, db, ci_tile, co_tile)
+    return (dw if ksize == k_out else dw[:, :, 1:2, 1:2].contiguous()), db
+
+
+# ------------------------------------------------------------------------------------------------
+# 8-bit activation checkpoints
+# ------------------------------------------------------------------------------------------------
+CHECKPOINT8_GROUP = 32
+_DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+
+
+class Checkpoint8(NamedTuple):
+    """What :func:`checkpoint8_pack` keeps of a (..., C) map: ``codes`` (..., C) float8_e4m3fn and ``scales``
+    (..., ceil(C / 32)) uint8, the byte s standing for the scale 2^(s - 127) of 32 channels; the map's value is code * scale,
+    exact in bf16 and fp32.  ``dtype``: the map's type; ``signbits``: its ReLU pattern, if asked for."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    dtype: torch.dtype
+    signbits: Optional[torch.Tensor] = None
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+
+def _dtype_code(dtype: torch.dtype, name: str) -> int:
+    if dtype not in _DTYPES:
+        raise TypeError(f"{name}: expected torch.bfloat16 or torch.float32, got {dtype}")
+    return _DTYPES[dtype]
+
+
+def _req_checkpoint8(ck: Checkpoint8, name: str):
+    """Contiguous (codes, scales) of a checkpoint whose parts belong together."""
+    codes, scales = _req(ck.codes, torch.float8_e4m3fn, f"{name}.codes"), _req(ck.scales, torch.uint8, f"{name}.scales")
+    _dtype_code(ck.dtype, f"{name}.dtype")
+    if codes.dim() < 1 or codes.shape[-1] < 1:
+        raise ValueError(f"{name}: a checkpoint has at least one channel")
+    if tuple(scales.shape) != tuple(codes.shape[:-1]) + ((codes.shape[-1] + CHECKPOINT8_GROUP - 1) // CHECKPOINT8_GROUP,):
+        raise ValueError(f"{name}: scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)}")
+    return codes, scales
+
+
+def checkpoint8_pack(x: torch.Tensor, signbits: bool = False) -> Checkpoint8:
+    """8-bit checkpoint of a (..., C) bf16 or fp32 map: e4m3 codes with a power-of-two scale per 32 channels, the smallest
+    that brings the group's largest finite magnitude to 448 or less; round to nearest even, a value that is not 0 keeps a
+    code that is not 0, infinities and NaN become NaN.  ``signbits=True`` ((N,H,W,64) bf16 maps): the same pass also writes
+    the ReLU pattern that the convolution's sign-bit forms read."""
+    dt = _dtype_code(x.dtype, "x")
+    x = _req(x, x.dtype, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("checkpoint8_pack: expected a (..., C) map with at least one channel")
+    c = x.shape[-1]
+    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty(tuple(x.shape[:-1]) + ((c + CHECKPOINT8_GROUP - 1) // CHECKPOINT8_GROUP,), dtype=torch.uint8, device=x.device)
+    bits = None
+    if signbits:
+        if x.dim() != 4 or c != 64 or x.dtype != torch.bfloat16:
+            raise ValueError("checkpoint8_pack: sign bits are kept of (N,H,W,64) bf16 maps")
+        n, h, w, _ = x.shape
+        bits = signbits_empty(n, h, w, x.device)
+        check(lib.srhip_checkpoint8_pack_signbits(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), bits.data_ptr(), n, h, w, _stream()))
+    else:
+        check(lib.srhip_checkpoint8_pack(x.data_ptr(), dt, codes.data_ptr(), scales.data_ptr(), x.numel() // c, c, _stream()))
+    return Checkpoint8(codes, scales, x.dtype, bits)
+
+
+def checkpoint8_restore(ck: Checkpoint8) -> torch.Tensor:
+    """The map that a checkpoint stands for, in the type of the one it was made from."""
+    codes, scales = _req_checkpoint8(ck, "ck")
+    y = torch.empty(codes.shape, dtype=ck.dtype, device=codes.device)
+    c = codes.shape[-1]
+    check(lib.srhip_checkpoint8_restore(codes.data_ptr(), scales.data_ptr(), y.data_ptr(), _DTYPES[ck.dtype], codes.numel() // c, c, _stream()))
+    return y
+
+
+def checkpoint8_wgrad(ck: Checkpoint8, dz: torch.Tensor, cin: int, cout: int, ksize: int = 3):
+    """:func:`conv_wgrad` of a layer whose input was kept as a checkpoint ((N,H,W,C), C a multiple of 16): the codes are decoded
+    on their way into the kernel, the result is that of the restored map bit for bit."""
+    return conv_wgrad((ck,), dz, cin, cout, ksize)
+
+
+def relu_mask(dy: torch.Tensor, y: Union[torch.Tensor, Checkpoint8], out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dy where y > 0 else 0 (bf16).  y may be a checkpoint of the map: the same pattern wherever y is finite."""
     dy = _req(dy, torch.bfloat16, "dy")
+    if isinstance(y, Checkpoint8):
+        codes, _ = _req_checkpoint8(y, "y")
+        if dy.shape != codes.shape:
+            raise ValueError("relu_mask: shapes differ")
+        if out is None:
+            out = torch.empty_like(dy)
+        elif out.dtype != torch.bfloat16 or out.shape != dy.shape or not out.is_contiguous() or out.device != dy.device:
+            raise ValueError("relu_mask: out must be a contiguous bf16 tensor of dy's shape")
+        check(lib.srhip_relu_mask_checkpoint8(dy.data_ptr(), codes.data_ptr(), out.data_ptr(), dy.numel(), _stream()))
+        return out
     y = _req(y, torch.bfloat16, "y")
     if dy.shape != y.shape:
         raise ValueError("relu_mask: shapes differ")
@@ -1124,6 +1284,174 @@ class _LayerNormCF(torch.autograd.Function):
 def layernorm_cf_autograd(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     """Differentiable channels-first LayerNorm (core/arch/CAMixerSR.py:29-37 under loss.backward())."""
     return _LayerNormCF.apply(x, weight, bias, eps)
+
+
+# ------------------------------------------------------------------------------------------------
+# the norms around a residual block, fused with its gate and residual scale
+# ------------------------------------------------------------------------------------------------
+NORM_MAX_CHANNELS = 8192
+_NORM_KINDS = {"layer": 0, "rms": 1}
+_GATE_ACTS = {"none": 0, "sigmoid": 1}
+_GATE_NONE, _GATE_ROWS, _GATE_MAP = 0, 1, 2
+
+
+class NormResidualGrads(NamedTuple):
+    """Gradients of :func:`norm_residual`; None for what the call does not have."""
+    dx: torch.Tensor
+    dh: Optional[torch.Tensor]
+    dpost_weight: Optional[torch.Tensor]
+    dpost_bias: Optional[torch.Tensor]
+    dgate: Optional[torch.Tensor]
+    dscale: Optional[torch.Tensor]
+    dpre_weight: Optional[torch.Tensor]
+    dpre_bias: Optional[torch.Tensor]
+
+
+def _norm_params(wb, c: int, name: str):
+    """(weight, bias or None) of one norm, or (None, None)."""
+    if wb is None:
+        return None, None
+    if not isinstance(wb, (tuple, list)) or len(wb) != 2 or wb[0] is None:
+        raise ValueError(f"{name}: expected (weight, bias or None)")
+    out = tuple(None if t is None else _req(t, torch.float32, f"{name} {k}") for t, k in zip(wb, ("weight", "bias")))
+    for t in out:
+        if t is not None and tuple(t.shape) != (c,):
+            raise ValueError(f"{name}: expected parameters of {c} channels, got {tuple(t.shape)}")
+    return out
+
+
+def _norm_gate(gate: Optional[torch.Tensor], like: torch.Tensor):
+    """(contiguous gate, mode, rows per gate, whether it is fp32 beside maps of another type)."""
+    if gate is None:
+        return None, _GATE_NONE, 0, 0
+    shape, c = tuple(like.shape), like.shape[-1]
+    rows = like.numel() // c
+    if tuple(gate.shape) == shape and gate.dtype in (like.dtype, torch.float32):
+        return _req(gate, gate.dtype, "gate"), _GATE_MAP, 0, int(gate.dtype != like.dtype)
+    if tuple(gate.shape) == (c,):
+        per = rows
+    elif like.dim() >= 3 and tuple(gate.shape) == (shape[0], c):
+        per = rows // max(1, shape[0])
+    else:
+        raise ValueError(f"gate: expected shape {(c,)}, {(shape[0], c)} or {shape} (of the maps' type or fp32), got {tuple(gate.shape)} {gate.dtype}")
+    gate = _req(gate, torch.float32, "gate")
+    if per == 1:   # one row to a gate: a map
+        return gate, _GATE_MAP, 0, int(like.dtype != torch.float32)
+    return gate, _GATE_ROWS, per, 0
+
+
+def _norm_scale(scale):
+    """(contiguous device scalar or None, its value where it is a number)."""
+    if isinstance(scale, torch.Tensor):
+        if scale.numel() != 1:
+            raise ValueError("scale: expected a number or a tensor of one element")
+        return _req(scale, torch.float32, "scale"), 0.0
+    return None, float(scale)
+
+
+def _norm_options(kind: str, gate_act: str, eps: float, c: int, name: str) -> None:
+    if kind not in _NORM_KINDS or gate_act not in _GATE_ACTS:
+        raise ValueError(f"{name}: kind is one of {sorted(_NORM_KINDS)}, gate_act one of {sorted(_GATE_ACTS)}; got {kind!r}, {gate_act!r}")
+    if not 1 <= c <= NORM_MAX_CHANNELS:
+        raise ValueError(f"{name}: 1 .. {NORM_MAX_CHANNELS} channels, got {c}")
+    if not eps >= 0.0:
+        raise ValueError(f"{name}: eps must not be negative")
+
+
+def norm_residual(x: torch.Tensor, h: Optional[torch.Tensor] = None, *, post=None, gate: Optional[torch.Tensor] = None, scale=1.0,
+                  pre=None, kind: str = "layer", gate_act: str = "none", eps: float = 1e-6):
+    """(r, n) with r = x + scale * gate_act(gate) * N_post(h) and n = N_pre(r), in one pass over (..., C) bf16 or fp32 maps: the
+    norm behind a residual block's branch, its gate and residual scale, the residual sum and the norm in front of the next
+    block.  All arithmetic in fp32; n is the norm of the sum before it is rounded to r.
+
+    post, pre: (weight, bias or None) of C fp32 values, or None: h itself is the branch / there is no n (None).
+    kind:      "layer" (v - mean) / sqrt(var + eps) * w + b, or "rms" v / sqrt(mean(v^2) + eps) * w + b, over the channels.
+    gate:      None; (C,) fp32; (N, C) fp32, a gate for each x[i]; or a map of x's shape, of its type or fp32.
+    gate_act:  "none" or "sigmoid".   scale: a number, or an fp32 tensor of one element.
+    h None:    only the norm, r is x itself."""
+    dt = _dtype_code(x.dtype, "x")
+    x = _req(x, x.dtype, "x")
+    if x.dim() < 2:
+        raise ValueError("norm_residual: expected a (..., C) map")
+    c = x.shape[-1]
+    _norm_options(kind, gate_act, eps, c, "norm_residual")
+    if h is None:
+        if pre is None or post is not None or gate is not None:
+            raise ValueError("norm_residual: without a branch there is only the norm `pre`")
+    else:
+        h = _req(h, x.dtype, "h")
+        if h.shape != x.shape:
+            raise ValueError("norm_residual: x and h differ in shape")
+    post_w, post_b = _norm_params(post, c, "post")
+    pre_w, pre_b = _norm_params(pre, c, "pre")
+    gate, mode, per, gate_f32 = _norm_gate(gate, x)
+    scale_t, scale_v = _norm_scale(scale)
+    r = x if h is None else torch.empty_like(x)
+    n = None if pre is None else torch.empty_like(x)
+    a = NormResidualArgs(x=x.data_ptr(), h=_ptr(h), gate=_ptr(gate), post_weight=_ptr(post_w), post_bias=_ptr(post_b), pre_weight=_ptr(pre_w),
+                         pre_bias=_ptr(pre_b), scale_ptr=_ptr(scale_t), r=_ptr(r), n=_ptr(n), rows=x.numel() // c, rows_per_gate=per, c=c, dtype=dt,
+                         kind=_NORM_KINDS[kind], post=int(post is not None), pre=int(pre is not None), gate_mode=mode, gate_f32=gate_f32,
+                         gate_sigmoid=_GATE_ACTS[gate_act], scale=scale_v, eps=eps)
+    check(lib.srhip_norm_residual_fwd(a, _stream()))
+    return r, n
+
+
+def norm_residual_bwd(h: Union[None, torch.Tensor, Checkpoint8], r: Union[None, torch.Tensor, Checkpoint8], dr: Optional[torch.Tensor],
+                      dn: Optional[torch.Tensor], *, post=None, gate: Optional[torch.Tensor] = None, scale=1.0, pre=None, kind: str = "layer",
+                      gate_act: str = "none", eps: float = 1e-6) -> NormResidualGrads:
+    """Gradients of :func:`norm_residual` from its h, its sum r and the gradients dr, dn of r and n (dr None: zero; dn goes with
+    ``pre``).  h and r may be checkpoints.  dx and dh have the maps' type, dgate the gate's, all others are fp32; dscale is
+    given where scale is a tensor, the biases' gradients where there are biases.  Sums over rows are taken in fp32 in a fixed
+    order (no atomics).  The norms' statistics are taken again, from r as it was rounded."""
+    like = dr if dr is not None else dn
+    if like is None or (pre is None) != (dn is None):
+        raise ValueError("norm_residual_bwd: needs dr or dn, and dn exactly where there is the norm `pre`")
+    dt = _dtype_code(like.dtype, "dr" if dr is not None else "dn")
+    dr = None if dr is None else _req(dr, like.dtype, "dr")
+    dn = None if dn is None else _req(dn, like.dtype, "dn")
+    if like.dim() < 2 or (dn is not None and dn.shape != like.shape):
+        raise ValueError("norm_residual_bwd: expected (..., C) maps of one shape")
+    c = like.shape[-1]
+    _norm_options(kind, gate_act, eps, c, "norm_residual_bwd")
+    if pre is not None and r is None:
+        raise ValueError("norm_residual_bwd: the norm `pre` needs r")
+    scale_t, scale_v = _norm_scale(scale)
+    if h is None and (post is not None or gate is not None or scale_t is not None):
+        raise ValueError("norm_residual_bwd: without a branch there is only the norm `pre`")
+
+    def saved(t, name):
+        if t is None:
+            return None, None
+        data, sc = _req_checkpoint8(t, name) if isinstance(t, Checkpoint8) else (_req(t, like.dtype, name), None)
+        if data.shape != like.shape or (sc is not None and t.dtype != like.dtype):
+            raise ValueError(f"norm_residual_bwd: {name} is not of the gradients' shape and type")
+        return data, sc
+
+    h_data, h_scales = saved(h, "h")
+    r_data, r_scales = saved(r if pre is not None else None, "r")
+    post_w, post_b = _norm_params(post, c, "post")
+    pre_w, pre_b = _norm_params(pre, c, "pre")
+    gate, mode, per, gate_f32 = _norm_gate(gate, like)
+    new = lambda t: None if t is None else torch.empty_like(t)  # noqa: E731
+    like = dr if dr is not None else dn
+    g = NormResidualGrads(torch.empty_like(like), torch.empty_like(like) if h is not None else None, new(post_w), new(post_b), new(gate), new(scale_t),
+                          new(pre_w), new(pre_b))
+    rows = like.numel() // c
+    if rows == 0:
+        for t in g:
+            if t is not None:
+                t.zero_()
+        return g
+    a = NormResidualBwdArgs(h=_ptr(h_data), h_scales=_ptr(h_scales), r=_ptr(r_data), r_scales=_ptr(r_scales), dr=_ptr(dr), dn=_ptr(dn), gate=_ptr(gate),
+                            post_weight=_ptr(post_w), post_bias=_ptr(post_b), pre_weight=_ptr(pre_w), scale_ptr=_ptr(scale_t), dx=_ptr(g.dx),
+                            dh=_ptr(g.dh), dgate=_ptr(g.dgate), dpost_weight=_ptr(g.dpost_weight), dpost_bias=_ptr(g.dpost_bias),
+                            dpre_weight=_ptr(g.dpre_weight), dpre_bias=_ptr(g.dpre_bias), dscale=_ptr(g.dscale), rows=rows, rows_per_gate=per, c=c,
+                            dtype=dt, kind=_NORM_KINDS[kind], post=int(post is not None), pre=int(pre is not None), gate_mode=mode, gate_f32=gate_f32,
+                            gate_sigmoid=_GATE_ACTS[gate_act], scale=scale_v, eps=eps)
+    ws = torch.empty((lib.srhip_norm_residual_bwd_workspace_bytes(a),), dtype=torch.uint8, device=like.device)
+    a.workspace = ws.data_ptr()
+    check(lib.srhip_norm_residual_bwd(a, _stream()))
+    return g
 
 
 # ------------------------------------------------------------------------------------------------
