@@ -11,6 +11,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import functional as F_
 
@@ -353,7 +354,7 @@ def _split_sources(dx: Tensor, srcs, cin: int, needs):
             if k0 == 0 and dx.shape[-1] == c:
                 out[i] = dx
             else:
-                d = torch.zeros_like(t)
+                d = torch.zeros(t.shape, dtype=dx.dtype, device=dx.device)
                 hi = min(k0 + c, dx.shape[-1])
                 d[..., :hi - k0] = dx[..., k0:hi]
                 out[i] = d
@@ -365,31 +366,40 @@ class _ConvReluChain(Function):
     """y_i = relu(conv_i(y_{i-1}) + b_i), i = 1..n, as ONE autograd node; y_0 may be several maps read as their
     concatenation.  The intermediate maps have no other consumer, so each intermediate ReLU backward rides on the
     data-gradient launch of the layer behind it (mask epilogue) instead of a pass of its own: one mask pass per chain.
-    Same launches, same roundings as n ``_ConvAuto`` nodes (a mask only zeroes): gradients are bit-equal."""
+    Same launches, same roundings as n ``_ConvAuto`` nodes (a mask only zeroes): gradients are bit-equal.
+    ``last_relu`` False: no activation behind the last layer.  ``checkpoint``: the sources and intermediate maps are kept as
+    8-bit checkpoints; data gradients stay the same, bit for bit, weight gradients are formed from the checkpoints."""
 
     @staticmethod
-    def forward(ctx, nsrc: int, cfgs, *tensors: Tensor):
+    def forward(ctx, nsrc: int, cfgs, last_relu: bool, checkpoint: bool, *tensors: Tensor):
         srcs, wb = tensors[:nsrc], tensors[nsrc:]
         ws = [w.detach().float().contiguous() for w in wb[0::2]]
         ys, x = [], (tuple(srcs) if nsrc > 1 else srcs[0])
-        for w, b, (stride, padding) in zip(ws, wb[1::2], cfgs):
+        for i, (w, b, (stride, padding)) in enumerate(zip(ws, wb[1::2], cfgs)):
             k = w.shape[-1]
             if b is None or w.shape[-2] != k or k not in (1, 3) or padding != k // 2 or stride not in (1, 2):
                 raise ValueError("autograd_ops.conv_relu_chain: layers are kernel 1 or 3 with padding kernel // 2, stride 1 or 2, with bias")
-            x = F_.conv2d_auto(x, w, b.detach().float().contiguous(), stride=stride, padding=padding, act=F_.ACT_RELU)
+            relu = last_relu or i + 1 < len(ws)
+            x = F_.conv2d_auto(x, w, b.detach().float().contiguous(), stride=stride, padding=padding, act=F_.ACT_RELU if relu else F_.ACT_NONE)
             ys.append(x)
-        ctx.save_for_backward(*srcs, *ys, *ws)
-        ctx.nsrc, ctx.cfgs = nsrc, tuple(cfgs)
-        return ys[-1]
+        last = ys.pop()
+        kept = [*srcs, *ys]
+        if checkpoint:
+            kept = [F_.checkpoint8_pack(t) for t in kept]
+        ctx.save_for_backward(*_saved_parts(kept), last if last_relu else None, *ws)
+        ctx.nsrc, ctx.cfgs, ctx.checkpoint = nsrc, tuple(cfgs), checkpoint
+        return last
 
     @staticmethod
     def backward(ctx, dy: Tensor):
         nsrc, cfgs = ctx.nsrc, ctx.cfgs
         n = len(cfgs)
         saved = ctx.saved_tensors
-        srcs, ys, ws = saved[:nsrc], saved[nsrc:nsrc + n], saved[nsrc + n:]
+        last, ws = saved[-n - 1], saved[-n:]
+        kept = _saved_maps(saved[:-n - 1], ctx.checkpoint)
+        srcs, ys = kept[:nsrc], kept[nsrc:]
         grads = [None] * (2 * n)
-        dz = F_.relu_mask(dy.contiguous(), ys[n - 1])
+        dz = dy.contiguous() if last is None else F_.relu_mask(dy.contiguous(), last)
         dsrcs = [None] * nsrc
         for i in range(n - 1, -1, -1):
             w = ws[i]
@@ -398,19 +408,87 @@ class _ConvReluChain(Function):
             dzs = dz if cfgs[i][0] == 1 else _zero_insert2(dz, h, wd)
             grads[2 * i], grads[2 * i + 1] = _auto_wgrad(inp, dzs, w)
             if i > 0:
-                dz = _auto_dgrad(dzs, w, mask=ys[i - 1])
+                dz = _auto_dgrad(dzs, w, mask=None if ctx.checkpoint else ys[i - 1])
                 if dz.shape[-1] != ys[i - 1].shape[-1]:
                     dz = _split_sources(dz, (ys[i - 1],), w.shape[1], (True,))[0]
-            elif any(ctx.needs_input_grad[2:2 + nsrc]):
-                dsrcs = _auto_dgrad_sources(dzs, w, srcs, ctx.needs_input_grad[2:2 + nsrc])
-        return (None, None) + tuple(dsrcs) + tuple(grads)
+                if ctx.checkpoint:
+                    dz = F_.relu_mask(dz, ys[i - 1], out=dz)
+            elif any(ctx.needs_input_grad[4:4 + nsrc]):
+                dsrcs = _auto_dgrad_sources(dzs, w, srcs, ctx.needs_input_grad[4:4 + nsrc])
+        return (None, None, None, None) + tuple(dsrcs) + tuple(grads)
 
 
-def conv_relu_chain(x, layers) -> Tensor:
-    """layers: [(weight, bias, stride, padding), ...], each followed by ReLU; x an NHWC bf16 map or a tuple of maps."""
+def _saved_parts(maps):
+    """The tensors of a list of maps, or of a list of checkpoints (codes, scales, codes, ...), for save_for_backward."""
+    return [t for m in maps for t in ((m.codes, m.scales) if isinstance(m, F_.Checkpoint8) else (m,))]
+
+
+def _saved_maps(tensors, checkpoint: bool, dtype: torch.dtype = torch.bfloat16):
+    return [F_.Checkpoint8(c, s, dtype) for c, s in zip(tensors[::2], tensors[1::2])] if checkpoint else list(tensors)
+
+
+def conv_relu_chain(x, layers, last_relu: bool = True, checkpoint: bool = False) -> Tensor:
+    """layers: [(weight, bias, stride, padding), ...], each followed by ReLU (the last: ``last_relu``); x an NHWC bf16 map or a
+    tuple of maps.  ``checkpoint``: what the backward pass needs of x and of the maps between the layers is kept in 8 bits (a
+    byte an element instead of two; functional.checkpoint8_pack)."""
     srcs = tuple(x) if isinstance(x, (tuple, list)) else (x,)
     flat = [t for (w, b, _, _) in layers for t in (w, b)]
-    return _ConvReluChain.apply(len(srcs), tuple((s, p) for (_, _, s, p) in layers), *srcs, *flat)
+    return _ConvReluChain.apply(len(srcs), tuple((s, p) for (_, _, s, p) in layers), last_relu, checkpoint, *srcs, *flat)
+
+
+class _NormResidual(Function):
+    """functional.norm_residual with its hand-written backward; ``cfg`` = (scale where it is a number, kind, gate_act, eps,
+    checkpoint).  Outputs: (r, n), r alone without a norm behind the sum, n alone without a branch."""
+
+    @staticmethod
+    def forward(ctx, x, h, gate, scale, post_w, post_b, pre_w, pre_b, cfg):
+        number, kind, gate_act, eps, checkpoint = cfg
+        how = dict(post=None if post_w is None else (post_w, post_b), gate=gate, scale=number if scale is None else scale,
+                   pre=None if pre_w is None else (pre_w, pre_b), kind=kind, gate_act=gate_act, eps=eps)
+        r, n = F_.norm_residual(x, h, **how)
+        # h is read again only where something behind it is differentiated, r only by the norm behind the sum
+        kept = [t for t, needed in ((h, h is not None and (post_w is not None or gate is not None or scale is not None)), (r, pre_w is not None)) if needed]
+        ctx.kept_h = len(kept) > (pre_w is not None)
+        if checkpoint:
+            kept = [F_.checkpoint8_pack(t) for t in kept]
+        ctx.nkept = len(kept)
+        ctx.save_for_backward(*_saved_parts(kept), gate, scale, post_w, post_b, pre_w, pre_b)
+        ctx.cfg, ctx.branch, ctx.dtype = cfg, h is not None, x.dtype
+        ctx.set_materialize_grads(False)
+        return n if h is None else r if n is None else (r, n)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        number, kind, gate_act, eps, checkpoint = ctx.cfg
+        saved = ctx.saved_tensors
+        gate, scale, post_w, post_b, pre_w, pre_b = saved[-6:]
+        dr, dn = (None, grads[0]) if not ctx.branch else (grads[0], grads[1] if len(grads) > 1 else None)
+        if dr is None and dn is None:
+            return (None,) * 9
+        kept = _saved_maps(saved[:-6], checkpoint, ctx.dtype)
+        like = dr if dr is not None else dn
+        # a branch that nothing reads again: any map of its shape says that there is one
+        h = None if not ctx.branch else kept[0] if ctx.kept_h else like
+        g = F_.norm_residual_bwd(h, kept[-1] if dn is not None else None, dr, dn, post=None if post_w is None else (post_w, post_b), gate=gate,
+                                 scale=number if scale is None else scale, pre=None if dn is None else (pre_w, pre_b), kind=kind, gate_act=gate_act,
+                                 eps=eps)
+        return g.dx, g.dh, g.dgate, g.dscale, g.dpost_weight, g.dpost_bias, g.dpre_weight, g.dpre_bias, None
+
+
+def norm_residual(x: Tensor, h: Optional[Tensor] = None, *, post=None, gate: Optional[Tensor] = None, scale=1.0, pre=None, kind: str = "layer",
+                  gate_act: str = "none", eps: float = 1e-6, checkpoint: bool = False):
+    """Differentiable functional.norm_residual: gradients for x, h, the gate, a scale that is a tensor and both norms' weights and
+    biases.  ``checkpoint``: what the backward pass needs of h and r is kept in 8 bits, the gradients are those at the kept
+    values (of the scale, the gate, the norms' parameters and inputs; the sum's own gradient passes through unchanged)."""
+    tensor = isinstance(scale, Tensor)
+    post_w, post_b = post if post is not None else (None, None)
+    pre_w, pre_b = pre if pre is not None else (None, None)
+    if h is None and tensor:
+        raise ValueError("norm_residual: without a branch there is only the norm `pre`")
+    out = _NormResidual.apply(x, h, gate, scale if tensor else None, post_w, post_b, pre_w, pre_b,
+                              (0.0 if tensor else float(scale), kind, gate_act, eps, checkpoint))
+    return (x, out) if h is None else out if pre is not None else (out, None)
 
 
 class _AttentionFuse(Function):

@@ -81,6 +81,9 @@ class SuperSampler(nn.Module):
         self.buffer_channels = buffer_channels
         self._init_parameters()
         self._packs: Dict[str, tuple] = {}
+        # training: keep the saved maps as 8-bit checkpoints (functional.checkpoint8_pack), about half the memory.  Output and data
+        # gradients do not change (the ReLU patterns are kept exactly); weight gradients are formed from maps of 3 mantissa bits
+        self.checkpoint_activations = False
         self.use_pair_kernel = os.environ.get("SRHIP_NO_PAIR", "0") != "1"
 
     def _init_parameters(self) -> None:
@@ -112,8 +115,8 @@ class SuperSampler(nn.Module):
     def _dgrad(self, name: str, conv: nn.Conv2d, dz: Tensor, lo: int = 0, n: int = None, mask: Tensor = None,
                res: Tensor = None, alpha: float = 1.0, signbits: Tensor = None, aux_mode: int = F_.AUX_NONE):
         """Gradient w.r.t. input channels [lo, lo+n) of ``conv`` from dz, the gradient of its pre-activation
-        output: alpha * conv_transpose(dz), then either masked by a saved ReLU output (``mask``) or added to
-        ``res``.  Runs the forward kernel on transposed, flipped weights.  With ``signbits`` (the 1-bit-per-element
+        output: alpha * conv_transpose(dz), then either masked by a saved ReLU output (``mask``, or its checkpoint in a pass of
+        its own) or added to ``res``.  Runs the forward kernel on transposed, flipped weights.  With ``signbits`` (the 1-bit-per-element
         ReLU pattern a forward launch emitted): ``AUX_MASKBITS`` masks the sum with ``res``, ``AUX_DUALBITS`` returns
         the gradient and its masked copy."""
         w = conv.weight
@@ -122,6 +125,9 @@ class SuperSampler(nn.Module):
             w.detach(), conv.out_channels, dz.shape[-1], cout=n, cout_off=lo, transpose_flip=True))
         if aux_mode != F_.AUX_NONE:
             return F_.conv3x3(dz, wp, None, n, res=res, act=F_.ACT_NONE, alpha=alpha, signbits=signbits, aux_mode=aux_mode)
+        if isinstance(mask, F_.Checkpoint8):
+            d = F_.conv3x3(dz, wp, None, n, res=res, act=F_.ACT_NONE, alpha=alpha)
+            return F_.relu_mask(d, mask, out=d)
         second = mask if mask is not None else res
         return F_.conv3x3(dz, wp, None, n, res=second, act=F_.ACT_NONE, alpha=alpha,
                           res_mode=F_.RES_MASK if mask is not None else F_.RES_ADD)

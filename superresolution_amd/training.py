@@ -11,6 +11,9 @@ autograd is done here layer by layer on NHWC bf16 tensors:
   * the 0.2 of ``SRResidualBlock`` (core/models/model.py:33) travels as ``alpha`` / ``scale``;
   * the up-sampling backward is a gather with the frame extractor's last ReLU fused.
 
+With ``model.checkpoint_activations`` the maps kept for the backward pass are 8-bit checkpoints (functional.Checkpoint8): the
+weight gradients read their codes, ReLU masks are the codes' signs.
+
 Master weights, gradients handed to the optimiser and the network output are fp32, activations and
 activation gradients bf16 (fp32 accumulation inside every kernel).
 """
@@ -56,6 +59,7 @@ class _SuperSamplerFn(torch.autograd.Function):
         prepared = hb.dtype == torch.bfloat16   # the HR trunk's input already as (B,th,tw,16) bf16 NHWC
         th, tw = hb.shape[1:3] if prepared else hb.shape[-2:]
         fc, bc, fr, bf, sr = m.frame_channels, m.buffer_channels, m.FR_CH, m.BF_CH, m.SR_CH
+        keep = F_.checkpoint8_pack if m.checkpoint_activations else lambda t: t   # what the backward pass gets of an HR map
         sv = {}
         # frame extractor @ LR (core/models/model.py:50-58,161)
         f = [F_.nchw_f32_to_nhwc_bf16(lr.float())]
@@ -82,29 +86,34 @@ class _SuperSamplerFn(torch.autograd.Function):
                 t1 = m._conv(f"ge{i + 1}a", blks[i + 1][0][0], x, bf)
                 t2 = m._conv(f"ge{i + 1}b", blks[i + 1][1][0], t1, bf)
                 nxt = F_.add_bf16(x, t2)
-            gb.append((prev, x, xbits, t1, t2))
+            gb.append((keep(prev), keep(x), xbits, keep(t1), t2 if bits else keep(t2)))
             prev, cin = nxt, bf
         g = prev
         # main trunk (model.py:82-95,169)
-        xs = [m._conv("main_in", m.main.conv_in[0], up, fr, xb=g, cin_b=bf)]
+        x_next = m._conv("main_in", m.main.conv_in[0], up, fr, xb=g, cin_b=bf)
         # the two-source launch cannot emit its ReLU pattern itself: one light pass (reads the map, writes 1/16 of it)
         # lets the backward mask inside the last data-gradient launch of the trunk
-        x0bits = F_.signbits_from_map(xs[0]) if (bits and sr == 64) else None
+        if m.checkpoint_activations:
+            xs = [F_.checkpoint8_pack(x_next, signbits=bits and sr == 64)]
+            x0bits = xs[0].signbits
+        else:
+            xs = [x_next]
+            x0bits = F_.signbits_from_map(xs[0]) if (bits and sr == 64) else None
         ts, tbits = [], []
         for i, blk in enumerate(m.main.conv_main):
             # one launch per block; the intermediate map is written out as well (the backward needs it), and from the
             # second block on its ReLU pattern too, in the form the block's one-launch backward reads (the first
             # block's backward folds conv_in's ReLU into its last launch instead and keeps two launches)
             if i >= 1:
-                x_next, t, tb = m._pair(f"m{i}", blk.blks[0], blk.blks[2], xs[-1], F_.ACT_NONE, 0.2, emit_bits=True)
+                x_next, t, tb = m._pair(f"m{i}", blk.blks[0], blk.blks[2], x_next, F_.ACT_NONE, 0.2, emit_bits=True)
             else:
-                (x_next, t), tb = m._pair(f"m{i}", blk.blks[0], blk.blks[2], xs[-1], F_.ACT_NONE, 0.2, keep_mid=True), None
-            ts.append(t)
+                (x_next, t), tb = m._pair(f"m{i}", blk.blks[0], blk.blks[2], x_next, F_.ACT_NONE, 0.2, keep_mid=True), None
+            ts.append(keep(t))
             tbits.append(tb)
-            xs.append(x_next)
-        a = m._conv("after", m.after_main[0], up, fr, xb=xs[-1], cin_b=sr)
+            xs.append(keep(x_next))
+        a = m._conv("after", m.after_main[0], up, fr, xb=x_next, cin_b=sr)
         out, c0 = m._pair_head("fin", m.final_conv[0], m.final_conv[2], a, keep_mid=True)   # one launch, c0 kept for the backward
-        sv.update(f=f, up=up, gb=gb, g=g, xs=xs, ts=ts, tbits=tbits, a=a, c0=c0, lr_hw=tuple(lr.shape[-2:]), bits=bits, x0bits=x0bits)
+        sv.update(f=f, up=keep(up), gb=gb, g=keep(g), xs=xs, ts=ts, tbits=tbits, a=keep(a), c0=keep(c0), lr_hw=tuple(lr.shape[-2:]), bits=bits, x0bits=x0bits)
         ctx.model, ctx.sv = m, sv
         return out
 

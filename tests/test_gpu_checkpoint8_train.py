@@ -1,0 +1,210 @@
+"""Checkpoints and the fused block norm where they are used: the default network's training step with its maps kept in 8 bits, and a
+residual block norm -> conv -> ReLU -> conv -> norm, gate, scale, sum -> norm under autograd."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _model(seed=0):
+    from superresolution_amd import SuperSampler
+    torch.manual_seed(seed)
+    m = SuperSampler(3, 10, 1).cuda()
+    with torch.no_grad():
+        for k, p in m.named_parameters():
+            if k.endswith("bias"):
+                p.normal_(std=0.05)
+    return m
+
+
+def _step(m, lr, hb, target):
+    m.zero_grad(set_to_none=True)
+    out = m({"lr_frames": lr, "hr_buffers": hb})["sr_frames"]
+    (out - target).abs().mean().backward()
+    return out.detach(), {k: p.grad.clone() for k, p in m.named_parameters()}
+
+
+def _batch(n, h, w, seed=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.rand(s, device="cuda", generator=g) for s in ((n, 1, 3, h, w), (n, 1, 10, 4 * h, 4 * w), (n, 3, 4 * h, 4 * w))]
+
+
+@pytest.mark.parametrize("signbits", ["0", "1"])
+def test_training_step_with_checkpoints_is_the_step_on_restored_maps(monkeypatch, signbits):
+    """Output, bias gradients and whatever comes from uncompressed maps do not change; the weight gradients are, bit for bit,
+    those of the same step whose saved maps were replaced by what their checkpoints stand for."""
+    from superresolution_amd import functional as F
+    monkeypatch.setenv("SRHIP_NO_SIGNBITS", signbits)
+    m, batch = _model(), _batch(2, 12, 23)
+    out, grads = _step(m, *batch)
+    m.checkpoint_activations = True
+    out8, grads8 = _step(m, *batch)
+    assert torch.equal(out, out8)
+    for k in grads:
+        if k.endswith("bias") or k.startswith("frame_extractor"):
+            assert torch.equal(grads[k], grads8[k]), k
+        else:
+            assert not torch.equal(grads[k], grads8[k]), k
+
+    pack = F.checkpoint8_pack
+
+    def restored(t, signbits=False):
+        ck = pack(t, signbits=signbits)
+        y = F.checkpoint8_restore(ck)
+        y.signbits = ck.signbits
+        return y
+
+    monkeypatch.setattr(F, "checkpoint8_pack", restored)
+    out_r, grads_r = _step(m, *batch)
+    assert torch.equal(out, out_r)
+    for k in grads:
+        assert torch.equal(grads8[k], grads_r[k]), k
+
+
+def test_checkpoints_keep_half_of_the_memory():
+    m, batch = _model(), _batch(2, 64, 64)
+    kept = []
+    for on in (False, True):
+        m.checkpoint_activations = on
+        _step(m, *batch)     # packed weights and workspaces exist
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = m({"lr_frames": batch[0], "hr_buffers": batch[1]})["sr_frames"]
+        kept.append(torch.cuda.memory_allocated() - before)
+        del out
+    # 33 bytes for 32 channels instead of 64 of every HR map; bit patterns, LR maps and the output stay: under 0.6
+    assert kept[1] < 0.6 * kept[0], kept
+
+
+def test_recurrent_network_trains_with_checkpoints():
+    from superresolution_amd import RecurrentSuperSampler
+    torch.manual_seed(0)
+    m = RecurrentSuperSampler(3, 10, 1).cuda()
+    lr, hb, target = _batch(1, 9, 17)
+    grads = []
+    for on in (False, True):
+        m.checkpoint_activations = on
+        grads.append(_step(m, lr, hb, target))
+    assert torch.equal(grads[0][0], grads[1][0])
+    assert all(torch.equal(grads[0][1][k], grads[1][1][k]) for k in grads[0][1] if k.endswith("bias"))
+
+
+# ---- a residual block
+def _block(x, p, c, checkpoint, gate):
+    from superresolution_amd import autograd_ops as A
+    _, n = A.norm_residual(x, pre=(p["n0w"], p["n0b"]), checkpoint=checkpoint)
+    h = A.conv_relu_chain(n, [(p["w1"], p["b1"], 1, 1), (p["w2"], p["b2"], 1, 1)], last_relu=False, checkpoint=checkpoint)
+    return A.norm_residual(x, h, post=(p["n1w"], p["n1b"]), gate=gate, gate_act="sigmoid", scale=p["scale"], pre=(p["n2w"], p["n2b"]), checkpoint=checkpoint)
+
+
+def _params(c, seed):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s, k=1.0: torch.randn(s, generator=g) * k  # noqa: E731
+    p = {"w1": n(c, c, 3, 3, k=0.06), "b1": n(c, k=0.1), "w2": n(c, c, 3, 3, k=0.06), "b2": n(c, k=0.1), "scale": torch.tensor(0.4)}
+    for i in range(3):
+        p[f"n{i}w"], p[f"n{i}b"] = 1 + n(c, k=0.2), n(c, k=0.2)
+    return {k: v.cuda().requires_grad_() for k, v in p.items()}
+
+
+def _reference(x, p, gate, on):
+    """The same block in 64 bits, nothing rounded between the operators.  ``on``: the ReLU pattern of the run it is compared
+    with.  A pre-activation whose rounding (relative error d) moves it across 0 is off by less than d, but switches a whole
+    gradient entry: a share of about 0.8 d of the entries, so sqrt(0.8 d) of the gradient's norm (0.05 for d = 2^-8.4), which
+    says nothing about the operators -- on either side of such a 0 the gradient is right."""
+    D = torch.float64
+    p = {k: v.detach().double().cpu().requires_grad_() for k, v in p.items()}
+    x, gate = x.detach().double().cpu().requires_grad_(), gate.detach().double().cpu().requires_grad_()
+    ln = lambda v, i: torch.nn.functional.layer_norm(v, v.shape[-1:], p[f"n{i}w"], p[f"n{i}b"], 1e-6)  # noqa: E731
+    conv = lambda v, i: torch.nn.functional.conv2d(v.permute(0, 3, 1, 2), p[f"w{i}"], p[f"b{i}"], padding=1).permute(0, 2, 3, 1)  # noqa: E731
+    h = conv(conv(ln(x, 0), 1) * on.double().cpu(), 2)
+    r = x + p["scale"] * torch.sigmoid(gate[:, None, None]) * ln(h, 1)
+    return x, gate, p, r, ln(r, 2)
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_a_residual_block_under_autograd(checkpoint):
+    from superresolution_amd import functional as F
+    c = 64
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(2, 11, 19, c, generator=g).bfloat16().cuda().requires_grad_()
+    gate = torch.randn(2, c, generator=g).cuda().requires_grad_()
+    dr, dn = (torch.randn(2, 11, 19, c, generator=g).bfloat16().cuda() for _ in range(2))
+    p = _params(c, 5)
+    r, n = _block(x, p, c, checkpoint, gate)
+    torch.autograd.backward((r, n), (dr, dn))
+    with torch.no_grad():
+        on = F.conv2d_auto(F.norm_residual(x, pre=(p["n0w"], p["n0b"]))[1], p["w1"], p["b1"], act=F.ACT_RELU) > 0
+    xr, gr, pr, rr, nr = _reference(x, p, gate, on)
+    torch.autograd.backward((rr, nr), (dr.double().cpu(), dn.double().cpu()))
+    # every map between the operators is rounded to bf16 (half a step: 2^-8) and the weights too: ten roundings in a row
+    # at most, each of them passed on by norms and convolutions that keep the size of what they are given, seen over the
+    # whole tensor: 10 * 2^-8.  A checkpoint's values are off by at most 2^-4 each, in what multiplies a gradient: 2^-4 more.
+    tol = 10 * 2.0 ** -8 + (2.0 ** -4 if checkpoint else 0.0)
+    rel = lambda a, b: float((a.detach().double().cpu() - b).norm() / b.norm())  # noqa: E731
+    assert rel(r, rr.detach()) < 10 * 2.0 ** -8 and rel(n, nr.detach()) < 10 * 2.0 ** -8
+    assert rel(x.grad, xr.grad) < tol and rel(gate.grad, gr.grad) < tol
+    for k in p:
+        assert rel(p[k].grad, pr[k].grad) < tol, k
+
+
+def test_checkpoints_of_a_chain_change_only_weight_gradients():
+    from superresolution_amd import autograd_ops as A
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(2, 14, 22, 96, generator=g).bfloat16().cuda()
+    shapes = [(112, 96, 1), (48, 112, 3), (64, 48, 3)]
+    layers = [((torch.randn(o, i, k, k, generator=g) * 0.1).cuda().requires_grad_(), torch.randn(o, generator=g).cuda().requires_grad_(), s, k // 2)
+              for (o, i, k), s in zip(shapes, (1, 2, 1))]
+    res = []
+    for ck in (False, True):
+        src = x.clone().requires_grad_()
+        for l in layers:
+            l[0].grad = l[1].grad = None
+        y = A.conv_relu_chain(src, layers, checkpoint=ck)
+        y.backward(torch.ones_like(y))
+        res.append((y.detach(), src.grad, [(l[0].grad, l[1].grad) for l in layers]))
+    plain, ck = res
+    assert torch.equal(plain[0], ck[0]) and torch.equal(plain[1], ck[1])
+    for (w0, b0), (w1, b1) in zip(plain[2], ck[2]):
+        assert torch.equal(b0, b1) and not torch.equal(w0, w1)
+        assert float((w0 - w1).norm() / w0.norm()) < 2.0 ** -4     # each value kept is off by at most 2^-4
+
+
+def test_autograd_forms_of_the_block_norm():
+    """Gradients through the autograd entry are the functional backward's; what is not asked for is not computed wrongly."""
+    from superresolution_amd import autograd_ops as A
+    from superresolution_amd import functional as F
+    g = torch.Generator().manual_seed(7)
+    n = lambda *s: torch.randn(s, generator=g).cuda()  # noqa: E731
+    x, h, w, b, w2 = n(3, 5, 40), n(3, 5, 40), n(40), n(40), n(40)
+    dr, dn = n(3, 5, 40), n(3, 5, 40)
+    leaf = lambda t: t.clone().requires_grad_()  # noqa: E731
+    # n alone is used, then r alone, then both
+    for use_r, use_n in ((False, True), (True, False), (True, True)):
+        lx, lh, lw, lb, lw2, s = leaf(x), leaf(h), leaf(w), leaf(b), leaf(w2), leaf(torch.tensor(0.3).cuda())
+        r, m = A.norm_residual(lx, lh, post=(lw, lb), scale=s, pre=(lw2, None), kind="rms")
+        loss = (r * dr).sum() * use_r + (m * dn).sum() * use_n if use_r and use_n else (r * dr).sum() if use_r else (m * dn).sum()
+        loss.backward()
+        want = F.norm_residual_bwd(h, r.detach(), dr if use_r else None, dn if use_n else None, post=(w, b), scale=torch.tensor(0.3).cuda(),
+                                   pre=(w2, None) if use_n else None, kind="rms")
+        assert torch.equal(lx.grad, want.dx) and torch.equal(lh.grad, want.dh) and torch.equal(s.grad, want.dscale)
+        assert torch.equal(lw.grad, want.dpost_weight) and torch.equal(lb.grad, want.dpost_bias)
+        assert (lw2.grad is None) if not use_n else torch.equal(lw2.grad, want.dpre_weight)
+    # a plain scaled sum: nothing of h is kept
+    lx, lh = leaf(x), leaf(h)
+    r, m = A.norm_residual(lx, lh, scale=0.2)
+    assert m is None
+    r.backward(dr)
+    assert torch.equal(lx.grad, dr) and torch.equal(lh.grad, 0.2 * dr)
+    # the norm alone, twice differentiated: refused, not silently wrong
+    lx = leaf(x)
+    r, m = A.norm_residual(lx, pre=(w, b))
+    assert r is lx
+    (d,) = torch.autograd.grad(m, lx, dn, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
+    # empty
+    e = torch.empty(0, 40, device="cuda", requires_grad=True)
+    A.norm_residual(e, e, pre=(w, b), checkpoint=True)[1].sum().backward()
+    assert e.grad.shape == e.shape
+    with pytest.raises(ValueError):
+        A.norm_residual(x, scale=torch.tensor(1.0).cuda(), pre=(w, b))
