@@ -52,35 +52,130 @@ struct RowSum {
 template <class C>
 constexpr int row_sum_scratch() { return C::TPR <= 64 ? 1 : 4 * C::RPB * (C::TPR / 64); }
 
-// mean (0 for the rms form) and 1 / sqrt(mean square of what is left + eps) of a row held as f[E]; elements from nv[v] on do
-// not exist and are 0.  Two sums over registers: the squares are taken of differences from the mean, as the definition has
-// it, so a mean that is large against the spread costs no digits.
+// What a lane holds of channels behind the row's end becomes 0.  Lanes that lie inside the row skip it: one branch.
 template <class C>
-__device__ __forceinline__ void row_statistics(RowSum<C>& sum, const float* f, const int* nv, const bool layer, const float inv_c, const float eps,
-                                               float& mean, float& rstd)
+__device__ __forceinline__ void zero_absent(float* f, const int* nv)
 {
-    mean = 0.0f;
-    if (layer) {
-        float s = 0.0f;
 #pragma unroll
-        for (int j = 0; j < C::E; ++j) s += f[j];
-        mean = sum.one(s) * inv_c;
-    }
-    float q = 0.0f;
+    for (int v = 0; v < C::V; ++v)
+        if (nv[v] < C::VEC)
 #pragma unroll
-    for (int j = 0; j < C::E; ++j) {
-        const float d = f[j] - mean;
-        q += j % C::VEC < nv[j / C::VEC] ? d * d : 0.0f;
-    }
-    rstd = 1.0f / sqrtf(sum.one(q) * inv_c + eps);
+            for (int k = 0; k < C::VEC; ++k)
+                if (k >= nv[v]) f[v * C::VEC + k] = 0.0f;
 }
 
-// `nv` floats of a parameter vector from channel c0 on; absent channels and an absent vector give `none`
+// Rows held as f[E] (absent channels 0) become (f - mean) / sqrt(mean square of that + eps), without the mean for the rms
+// form; returns the factor 1 / sqrt.  Two sums over registers: the squares are taken of differences from the mean, as the
+// definition has it, so a mean that is large against the spread costs no digits.  Two rows at once share their sums' steps.
 template <class C>
-__device__ __forceinline__ void load_params(const float* p, const int c0, const int nv, const float none, float* f)
+__device__ __forceinline__ void normalise(RowSum<C>& sum, const bool first, float* f, const bool second, float* g, const int* nv, const bool layer,
+                                          const float inv_c, const float eps, float& rstd_f, float& rstd_g)
+{
+    float a = 0.0f, b = 0.0f;
+    if (layer) {
+        if (first)
+#pragma unroll
+            for (int j = 0; j < C::E; ++j) a += f[j];
+        if (second)
+#pragma unroll
+            for (int j = 0; j < C::E; ++j) b += g[j];
+        sum.two(a, b);
+        a *= inv_c;
+        b *= inv_c;
+        if (first) {
+#pragma unroll
+            for (int j = 0; j < C::E; ++j) f[j] -= a;
+            zero_absent<C>(f, nv);
+        }
+        if (second) {
+#pragma unroll
+            for (int j = 0; j < C::E; ++j) g[j] -= b;
+            zero_absent<C>(g, nv);
+        }
+        a = b = 0.0f;
+    }
+    if (first)
+#pragma unroll
+        for (int j = 0; j < C::E; ++j) a += f[j] * f[j];
+    if (second)
+#pragma unroll
+        for (int j = 0; j < C::E; ++j) b += g[j] * g[j];
+    sum.two(a, b);
+    rstd_f = 1.0f / sqrtf(a * inv_c + eps);
+    rstd_g = 1.0f / sqrtf(b * inv_c + eps);
+    if (first)
+#pragma unroll
+        for (int j = 0; j < C::E; ++j) f[j] *= rstd_f;
+    if (second)
+#pragma unroll
+        for (int j = 0; j < C::E; ++j) g[j] *= rstd_g;
+}
+template <class C>
+__device__ __forceinline__ float normalise(RowSum<C>& sum, float* f, const int* nv, const bool layer, const float inv_c, const float eps)
+{
+    float a = 0.0f;
+    if (layer) {
+#pragma unroll
+        for (int j = 0; j < C::E; ++j) a += f[j];
+        a = sum.one(a) * inv_c;
+#pragma unroll
+        for (int j = 0; j < C::E; ++j) f[j] -= a;
+        zero_absent<C>(f, nv);
+        a = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < C::E; ++j) a += f[j] * f[j];
+    const float rstd = 1.0f / sqrtf(sum.one(a) * inv_c + eps);
+#pragma unroll
+    for (int j = 0; j < C::E; ++j) f[j] *= rstd;
+    return rstd;
+}
+
+// A parameter vector's values of a lane's channels: `none` where there is no vector, 0 for absent channels.
+template <class C>
+__device__ __forceinline__ void load_params(const float* p, const int* c0, const int* nv, const float none, float* f)
 {
 #pragma unroll
-    for (int j = 0; j < C::VEC; ++j) f[j] = p != nullptr && j < nv ? p[c0 + j] : none;
+    for (int v = 0; v < C::V; ++v)
+#pragma unroll
+        for (int j = 0; j < C::VEC; ++j) f[v * C::VEC + j] = j < nv[v] ? (p != nullptr ? p[c0[v] + j] : none) : 0.0f;
+}
+// A map's row, or part of it.  `whole`: no lane's vector reaches past the row's end (one test for the launch).
+template <class C>
+__device__ __forceinline__ void load_row(const char* p, const int* c0, const int* nv, const bool whole, rows_u32x4* q)
+{
+    using T = typename C::T;
+    if (whole) {
+#pragma unroll
+        for (int v = 0; v < C::V; ++v) q[v] = load16(p + c0[v] * RowVec<T>::SIZE);
+    } else {
+#pragma unroll
+        for (int v = 0; v < C::V; ++v) q[v] = load_row16<T>(p + c0[v] * RowVec<T>::SIZE, nv[v]);
+    }
+}
+template <class C>
+__device__ __forceinline__ void store_row(char* p, const int* c0, const int* nv, const bool whole, const float* f)
+{
+    using T = typename C::T;
+    if (whole) {
+#pragma unroll
+        for (int v = 0; v < C::V; ++v) store16(p + c0[v] * RowVec<T>::SIZE, RowVec<T>::pack(f + v * C::VEC));
+    } else {
+#pragma unroll
+        for (int v = 0; v < C::V; ++v) store_row16<T>(p + c0[v] * RowVec<T>::SIZE, RowVec<T>::pack(f + v * C::VEC), nv[v]);
+    }
+}
+template <class C>
+__device__ __forceinline__ void unpack_row(const rows_u32x4* q, float* f)
+{
+#pragma unroll
+    for (int v = 0; v < C::V; ++v) RowVec<typename C::T>::unpack(q[v], f + v * C::VEC);
+}
+// the gate map's row where it is fp32 beside bf16 maps
+template <class C>
+__device__ __forceinline__ void load_gate_f32(const char* p, const int* c0, const int* nv, float* g)
+{
+    load_params<C>((const float*)p, c0, nv, 0.0f, g);
 }
 
 __device__ __forceinline__ float sigmoid_f32(const float x) { return 1.0f / (1.0f + expf(-x)); }

@@ -25,94 +25,83 @@ struct NormParams {
     float scale, eps, inv_c;
 };
 
-template <class C>
+// MAPG: the gate is a map.  Otherwise it is constant over runs of rows and sits, times the scale, in the post norm's parameters.
+template <class C, bool MAPG>
 __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormParams p)
 {
     using T = typename C::T;
-    constexpr int SIZE = RowVec<T>::SIZE, VEC = C::VEC;
+    constexpr int SIZE = RowVec<T>::SIZE, VEC = C::VEC, E = C::E;
     __shared__ float scratch[row_sum_scratch<C>()];
     RowSum<C> sum{scratch, 0};
     const int t = threadIdx.x % C::TPR, rg = threadIdx.x / C::TPR;
+    const bool whole = p.c == C::CMAX;
     int c0[C::V], nv[C::V];
-    float wpost[C::E], bpost[C::E], wpre[C::E], bpre[C::E], g[C::E];
 #pragma unroll
     for (int v = 0; v < C::V; ++v) {
         c0[v] = (v * C::TPR + t) * VEC;
         nv[v] = p.c - c0[v];
-        load_params<C>(p.post_w, c0[v], nv[v], 1.0f, wpost + v * VEC);
-        load_params<C>(p.post_b, c0[v], nv[v], 0.0f, bpost + v * VEC);
-        load_params<C>(p.pre_w, c0[v], nv[v], 1.0f, wpre + v * VEC);
-        load_params<C>(p.pre_b, c0[v], nv[v], 0.0f, bpre + v * VEC);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) g[v * VEC + j] = 1.0f;
     }
+    float wpost[E], bpost[E], wpre[E], bpre[E];
+    load_params<C>(p.pre_w, c0, nv, 1.0f, wpre);
+    load_params<C>(p.pre_b, c0, nv, 0.0f, bpre);
     const float scale = p.scale_ptr ? *p.scale_ptr : p.scale;
     long long gate_end = 0;   // first row that the gate held in registers does not belong to
+    if (p.gate_mode != SRHIP_GATE_ROWS) {
+        load_params<C>(p.post_w, c0, nv, 1.0f, wpost);
+        load_params<C>(p.post_b, c0, nv, 0.0f, bpost);
+#pragma unroll
+        for (int j = 0; j < E; ++j) { wpost[j] *= scale; bpost[j] *= scale; }
+    }
 
     for (long long base = (long long)blockIdx.x * C::RPB; base < p.rows; base += (long long)gridDim.x * C::RPB) {
         const bool live = base + rg < p.rows;
         const long long row = live ? base + rg : p.rows - 1;   // lanes behind the last row work on it too and store nothing
-        const long long at = row * p.c;
+        const long long at = row * p.c * SIZE;
         rows_u32x4 qx[C::V], qh[C::V], qg[C::V];
-#pragma unroll
-        for (int v = 0; v < C::V; ++v) qx[v] = load_row16<T>(p.x + (at + c0[v]) * SIZE, nv[v]);
-        if (p.h)
-#pragma unroll
-            for (int v = 0; v < C::V; ++v) qh[v] = load_row16<T>(p.h + (at + c0[v]) * SIZE, nv[v]);
-        if (p.gate_mode == SRHIP_GATE_MAP) {
-            if (p.gate_f32) {
-#pragma unroll
-                for (int v = 0; v < C::V; ++v) load_params<C>((const float*)p.gate + at, c0[v], nv[v], 0.0f, g + v * VEC);
-            } else {
-#pragma unroll
-                for (int v = 0; v < C::V; ++v) qg[v] = load_row16<T>(p.gate + (at + c0[v]) * SIZE, nv[v]);
-#pragma unroll
-                for (int v = 0; v < C::V; ++v) RowVec<T>::unpack(qg[v], g + v * VEC);
-            }
+        float g[E];
+        load_row<C>(p.x + at, c0, nv, whole, qx);
+        if (p.h) load_row<C>(p.h + at, c0, nv, whole, qh);
+        if constexpr (MAPG) {
+            if (p.gate_f32) load_gate_f32<C>(p.gate + row * p.c * 4, c0, nv, g);
+            else load_row<C>(p.gate + at, c0, nv, whole, qg);
         } else if (p.gate_mode == SRHIP_GATE_ROWS && row >= gate_end) {   // rows of a lane only grow
             const long long s = row / p.rows_per_gate;
             gate_end = (s + 1) * p.rows_per_gate;
+            load_params<C>((const float*)p.gate + s * p.c, c0, nv, 0.0f, g);
+            load_params<C>(p.post_w, c0, nv, 1.0f, wpost);
+            load_params<C>(p.post_b, c0, nv, 0.0f, bpost);
 #pragma unroll
-            for (int v = 0; v < C::V; ++v) load_params<C>((const float*)p.gate + s * p.c, c0[v], nv[v], 0.0f, g + v * VEC);
-            if (p.sigmoid)
-#pragma unroll
-                for (int j = 0; j < C::E; ++j) g[j] = sigmoid_f32(g[j]);
+            for (int j = 0; j < E; ++j) {
+                const float f = scale * (p.sigmoid ? sigmoid_f32(g[j]) : g[j]);
+                wpost[j] *= f;
+                bpost[j] *= f;
+            }
         }
-        if (p.gate_mode == SRHIP_GATE_MAP && p.sigmoid)
-#pragma unroll
-            for (int j = 0; j < C::E; ++j) g[j] = sigmoid_f32(g[j]);
 
-        float r[C::E];
-#pragma unroll
-        for (int v = 0; v < C::V; ++v) RowVec<T>::unpack(qx[v], r + v * VEC);
+        float r[E];
+        unpack_row<C>(qx, r);
         if (p.h) {
-            float h[C::E];
+            float h[E];
+            unpack_row<C>(qh, h);
+            if (p.post) normalise<C>(sum, h, nv, p.layer, p.inv_c, p.eps);
+            if constexpr (MAPG) {
+                if (!p.gate_f32) unpack_row<C>(qg, g);
+                if (p.sigmoid)
 #pragma unroll
-            for (int v = 0; v < C::V; ++v) RowVec<T>::unpack(qh[v], h + v * VEC);
-            if (p.post) {
-                float mean, rstd;
-                row_statistics<C>(sum, h, nv, p.layer, p.inv_c, p.eps, mean, rstd);
+                    for (int j = 0; j < E; ++j) g[j] = sigmoid_f32(g[j]);
 #pragma unroll
-                for (int j = 0; j < C::E; ++j) h[j] = (h[j] - mean) * rstd * wpost[j] + bpost[j];
+                for (int j = 0; j < E; ++j) r[j] += g[j] * (h[j] * wpost[j] + bpost[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < E; ++j) r[j] += h[j] * wpost[j] + bpost[j];
             }
-#pragma unroll
-            for (int v = 0; v < C::V; ++v) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    const int j = v * VEC + k;
-                    r[j] = k < nv[v] ? r[j] + scale * (g[j] * h[j]) : 0.0f;
-                }
-                if (live) store_row16<T>(p.r + (at + c0[v]) * SIZE, RowVec<T>::pack(r + v * VEC), nv[v]);
-            }
+            if (live) store_row<C>(p.r + at, c0, nv, whole, r);
         }
         if (p.pre) {
-            float mean, rstd;
-            row_statistics<C>(sum, r, nv, p.layer, p.inv_c, p.eps, mean, rstd);
+            normalise<C>(sum, r, nv, p.layer, p.inv_c, p.eps);
 #pragma unroll
-            for (int j = 0; j < C::E; ++j) r[j] = (r[j] - mean) * rstd * wpre[j] + bpre[j];
-            if (live)
-#pragma unroll
-                for (int v = 0; v < C::V; ++v) store_row16<T>(p.n + (at + c0[v]) * SIZE, RowVec<T>::pack(r + v * VEC), nv[v]);
+            for (int j = 0; j < E; ++j) r[j] = r[j] * wpre[j] + bpre[j];
+            if (live) store_row<C>(p.n + at, c0, nv, whole, r);
         }
     }
 }
@@ -123,7 +112,9 @@ int launch(const NormParams& p, hipStream_t stream)
     // as many work-groups as are resident at once: each keeps its parameters in registers over all its rows
     const long long want = (p.rows + C::RPB - 1) / C::RPB;
     const long long resident = (long long)srhip_num_cus() * (2048 / C::THREADS);
-    hipLaunchKernelGGL(norm_residual_kernel<C>, dim3((unsigned)(want < resident ? want : resident)), dim3(C::THREADS), 0, stream, p);
+    const dim3 grid((unsigned)(want < resident ? want : resident));
+    if (p.gate_mode == SRHIP_GATE_MAP) hipLaunchKernelGGL((norm_residual_kernel<C, true>), grid, dim3(C::THREADS), 0, stream, p);
+    else hipLaunchKernelGGL((norm_residual_kernel<C, false>), grid, dim3(C::THREADS), 0, stream, p);
     return srhip_check_launch("norm_residual_kernel");
 }
 

@@ -125,6 +125,24 @@ __device__ __forceinline__ float lanes_sum(const float v)
 {
     return lanes_reduce<W>(v, [](float a, float b) { return a + b; });
 }
+// Sum over the lanes of a wave that have the same place in their group of W lanes; every lane gets it.
+template <int W>
+__device__ __forceinline__ float same_place_sum(float v)
+{
+    if constexpr (W <= 1) v += dpp_move<0xB1>(v);
+    if constexpr (W <= 2) v += dpp_move<0x4E>(v);     // the other pair of each quad
+    if constexpr (W <= 4) v += dpp_move<0x124>(v);    // rotate sixteen lanes by 4, then by 8: all four quads
+    if constexpr (W <= 8) v += dpp_move<0x128>(v);
+    if constexpr (W <= 16) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    if constexpr (W <= 32) {
+        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    return v;
+}
 template <int W>
 __device__ __forceinline__ float lanes_max(const float v)
 {
