@@ -9,6 +9,8 @@
 // n is the norm of the unrounded sum.  All arithmetic in fp32, each output rounded once.
 //
 // Bound by HBM: x, h (and a gate map) are read once, r and n written once, a row stays in the registers of its lanes.
+#include <atomic>
+
 #include "norm_residual.h"
 
 namespace {
@@ -21,6 +23,7 @@ struct NormParams {
     char* r;
     char* n;
     long long rows, rows_per_gate;
+    long long wg_rows, wg_step;   // a work-group takes wg_rows rows, or (wg_step > 0) wg_rows of every wg_step
     int c, layer, post, pre, gate_mode, gate_f32, sigmoid;
     float scale, eps, inv_c;
 };
@@ -53,7 +56,8 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormPar
         for (int j = 0; j < E; ++j) { wpost[j] *= scale; bpost[j] *= scale; }
     }
 
-    for (long long base = (long long)blockIdx.x * C::RPB; base < p.rows; base += (long long)gridDim.x * C::RPB) {
+    const long long first = blockIdx.x * p.wg_rows, last = p.wg_rows < p.rows - first ? first + p.wg_rows : p.rows;
+    for (long long base = first; base < (p.wg_step ? p.rows : last); base += p.wg_step ? p.wg_step : C::RPB) {
         const bool live = base + rg < p.rows;
         const long long row = live ? base + rg : p.rows - 1;   // lanes behind the last row work on it too and store nothing
         const long long at = row * p.c * SIZE;
@@ -106,16 +110,40 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormPar
     }
 }
 
+template <class C, bool MAPG>
+int launch_rows(NormParams p, hipStream_t stream)
+{
+    const long long passes = (p.rows + C::RPB - 1) / C::RPB;
+    long long grid;
+    if (C::TPR <= 64 && C::E <= 8) {
+        // Short rows: eight passes to a work-group, enough to pay for its parameters, and as many work-groups as that makes
+        // (64 channels of four 1024^2 crops: 389 us; 4, 16, 32 passes 436, 412, 433 us; work-groups that stay resident and
+        // stride over the rows 432 us).
+        p.wg_rows = 8 * C::RPB;
+        p.wg_step = 0;
+        grid = (passes + 7) / 8;
+    } else {
+        // Long rows: the work-groups that fit the device at once stride over the rows (16000 rows of 4096: 108 us, of eight
+        // rows to a work-group 125 us: the last of them leave the device half empty).
+        static std::atomic<int> fit[kSrhipMaxDevices];
+        const int dev = srhip_current_device();
+        int n = fit[dev].load(std::memory_order_relaxed);
+        if (n == 0) {
+            if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, norm_residual_kernel<C, MAPG>, C::THREADS, 0) != hipSuccess || n < 1) n = 1;
+            fit[dev].store(n, std::memory_order_relaxed);
+        }
+        grid = (long long)srhip_num_cus() * n < passes ? (long long)srhip_num_cus() * n : passes;
+        p.wg_rows = C::RPB;
+        p.wg_step = grid * C::RPB;
+    }
+    SRHIP_REQUIRE(grid < (1ll << 31), "norm_residual: too many rows");
+    hipLaunchKernelGGL((norm_residual_kernel<C, MAPG>), dim3((unsigned)grid), dim3(C::THREADS), 0, stream, p);
+    return srhip_check_launch("norm_residual_kernel");
+}
 template <class C>
 int launch(const NormParams& p, hipStream_t stream)
 {
-    // as many work-groups as are resident at once: each keeps its parameters in registers over all its rows
-    const long long want = (p.rows + C::RPB - 1) / C::RPB;
-    const long long resident = (long long)srhip_num_cus() * (2048 / C::THREADS);
-    const dim3 grid((unsigned)(want < resident ? want : resident));
-    if (p.gate_mode == SRHIP_GATE_MAP) hipLaunchKernelGGL((norm_residual_kernel<C, true>), grid, dim3(C::THREADS), 0, stream, p);
-    else hipLaunchKernelGGL((norm_residual_kernel<C, false>), grid, dim3(C::THREADS), 0, stream, p);
-    return srhip_check_launch("norm_residual_kernel");
+    return p.gate_mode == SRHIP_GATE_MAP ? launch_rows<C, true>(p, stream) : launch_rows<C, false>(p, stream);
 }
 
 // the narrowest group of lanes that holds a row
