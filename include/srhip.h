@@ -649,7 +649,8 @@ SRHIP_API int srhip_norm_residual_fwd(const srhip_norm_residual_args* args, void
  *   dgate        SRHIP_GATE_ROWS: fp32 (rows / rows_per_gate, c);  SRHIP_GATE_MAP: of the gate's type
  *   dscale       fp32 on the device, or NULL
  *   d*_bias      fp32[c] or NULL
- *   workspace    srhip_norm_residual_bwd_workspace_bytes(args) bytes (a function of rows, rows_per_gate, c and gate_mode)
+ *   workspace    srhip_norm_residual_bwd_workspace_bytes(args) bytes (a function of rows, rows_per_gate, c, dtype, gate_mode and of
+ *                whether h_scales, r_scales are NULL)
  * rows >= 1.  Deterministic: sums over rows are added in a fixed order, without atomics. */
 typedef struct {
     const void* h;

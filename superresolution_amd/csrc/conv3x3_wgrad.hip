@@ -184,10 +184,10 @@ __device__ __forceinline__ void decode_to_lds(const rows_u32x4 q, const float sc
     rows_u32x4 lo, hi;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        float f[4];
-        ck8_unpack4(q[j], scale, f);
-        (j < 2 ? lo : hi)[2 * (j & 1)] = pack_bf16x2(f[0], f[1]);
-        (j < 2 ? lo : hi)[2 * (j & 1) + 1] = pack_bf16x2(f[2], f[3]);
+        unsigned a, b;
+        ck8_unpack4_bf16(q[j], scale, a, b);
+        (j < 2 ? lo : hi)[2 * (j & 1)] = a;
+        (j < 2 ? lo : hi)[2 * (j & 1) + 1] = b;
     }
     asm volatile("ds_write_b128 %0, %1\n\tds_write_b128 %0, %2 offset:16" ::"v"(addr), "v"(lo), "v"(hi) : "memory");
 }

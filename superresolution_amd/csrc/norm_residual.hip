@@ -32,48 +32,41 @@ struct NormParams {
 template <class C, bool MAPG>
 __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormParams p)
 {
-    using T = typename C::T;
-    constexpr int SIZE = RowVec<T>::SIZE, VEC = C::VEC, E = C::E;
+    constexpr int SIZE = C::SIZE, E = C::E;
     __shared__ float scratch[row_sum_scratch<C>()];
     RowSum<C> sum{scratch, 0};
-    const int t = threadIdx.x % C::TPR, rg = threadIdx.x / C::TPR;
-    const bool whole = p.c == C::CMAX;
-    int c0[C::V], nv[C::V];
-#pragma unroll
-    for (int v = 0; v < C::V; ++v) {
-        c0[v] = (v * C::TPR + t) * VEC;
-        nv[v] = p.c - c0[v];
-    }
+    const Lane<C> l(p.c);
     float wpost[E], bpost[E], wpre[E], bpre[E];
-    load_params<C>(p.pre_w, c0, nv, 1.0f, wpre);
-    load_params<C>(p.pre_b, c0, nv, 0.0f, bpre);
+    load_params<C>(p.pre_w, l, 1.0f, wpre);
+    load_params<C>(p.pre_b, l, 0.0f, bpre);
     const float scale = p.scale_ptr ? *p.scale_ptr : p.scale;
     long long gate_end = 0;   // first row that the gate held in registers does not belong to
     if (p.gate_mode != SRHIP_GATE_ROWS) {
-        load_params<C>(p.post_w, c0, nv, 1.0f, wpost);
-        load_params<C>(p.post_b, c0, nv, 0.0f, bpost);
+        load_params<C>(p.post_w, l, 1.0f, wpost);
+        load_params<C>(p.post_b, l, 0.0f, bpost);
 #pragma unroll
         for (int j = 0; j < E; ++j) { wpost[j] *= scale; bpost[j] *= scale; }
     }
 
-    const long long first = blockIdx.x * p.wg_rows, last = p.wg_rows < p.rows - first ? first + p.wg_rows : p.rows;
-    for (long long base = first; base < (p.wg_step ? p.rows : last); base += p.wg_step ? p.wg_step : C::RPB) {
-        const bool live = base + rg < p.rows;
-        const long long row = live ? base + rg : p.rows - 1;   // lanes behind the last row work on it too and store nothing
-        const long long at = row * p.c * SIZE;
+    const long long first = blockIdx.x * p.wg_rows, last = p.wg_step || p.wg_rows > p.rows - first ? p.rows : first + p.wg_rows;
+    for (long long base = first; base < last; base += p.wg_step ? p.wg_step : C::RPB) {
+        // lanes behind the last row work on it too and store nothing
+        const bool live = l.rg < p.rows - base;
+        const unsigned back = live ? 0u : (unsigned)((l.rg - (int)(p.rows - base - 1)) * p.c);
+        const long long at = base * p.c * SIZE;
         rows_u32x4 qx[C::V], qh[C::V], qg[C::V];
         float g[E];
-        load_row<C>(p.x + at, c0, nv, whole, qx);
-        if (p.h) load_row<C>(p.h + at, c0, nv, whole, qh);
+        load_row<C>(p.x + at, l, back, qx);
+        if (p.h) load_row<C>(p.h + at, l, back, qh);
         if constexpr (MAPG) {
-            if (p.gate_f32) load_gate_f32<C>(p.gate + row * p.c * 4, c0, nv, g);
-            else load_row<C>(p.gate + at, c0, nv, whole, qg);
-        } else if (p.gate_mode == SRHIP_GATE_ROWS && row >= gate_end) {   // rows of a lane only grow
-            const long long s = row / p.rows_per_gate;
+            if (p.gate_f32) load_gate_f32<C>(p.gate + base * p.c * 4, l, back, g);
+            else load_row<C>(p.gate + at, l, back, qg);
+        } else if (p.gate_mode == SRHIP_GATE_ROWS && live && base + l.rg >= gate_end) {   // rows of a lane only grow
+            const long long s = (base + l.rg) / p.rows_per_gate;
             gate_end = (s + 1) * p.rows_per_gate;
-            load_params<C>((const float*)p.gate + s * p.c, c0, nv, 0.0f, g);
-            load_params<C>(p.post_w, c0, nv, 1.0f, wpost);
-            load_params<C>(p.post_b, c0, nv, 0.0f, bpost);
+            load_params<C>((const float*)p.gate + s * p.c, l, 0.0f, g);
+            load_params<C>(p.post_w, l, 1.0f, wpost);
+            load_params<C>(p.post_b, l, 0.0f, bpost);
 #pragma unroll
             for (int j = 0; j < E; ++j) {
                 const float f = scale * (p.sigmoid ? sigmoid_f32(g[j]) : g[j]);
@@ -87,7 +80,7 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormPar
         if (p.h) {
             float h[E];
             unpack_row<C>(qh, h);
-            if (p.post) normalise<C>(sum, h, nv, p.layer, p.inv_c, p.eps);
+            if (p.post) normalise<C>(sum, l, h, p.layer, p.inv_c, p.eps);
             if constexpr (MAPG) {
                 if (!p.gate_f32) unpack_row<C>(qg, g);
                 if (p.sigmoid)
@@ -99,13 +92,13 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormPar
 #pragma unroll
                 for (int j = 0; j < E; ++j) r[j] += h[j] * wpost[j] + bpost[j];
             }
-            if (live) store_row<C>(p.r + at, c0, nv, whole, r);
+            if (live) store_row<C>(p.r + at, l, r);
         }
         if (p.pre) {
-            normalise<C>(sum, r, nv, p.layer, p.inv_c, p.eps);
+            normalise<C>(sum, l, r, p.layer, p.inv_c, p.eps);
 #pragma unroll
             for (int j = 0; j < E; ++j) r[j] = r[j] * wpre[j] + bpre[j];
-            if (live) store_row<C>(p.n + at, c0, nv, whole, r);
+            if (live) store_row<C>(p.n + at, l, r);
         }
     }
 }
@@ -147,20 +140,26 @@ int launch(const NormParams& p, hipStream_t stream)
 }
 
 // the narrowest group of lanes that holds a row
-template <class T>
+template <class T, bool ODD>
 int dispatch(const NormParams& p, hipStream_t s)
 {
     constexpr int K = 8 / RowVec<T>::VEC;   // vectors for 8 channels
-    if (p.c <= 16) return launch<RowCfg<T, 2, K>>(p, s);
-    if (p.c <= 32) return launch<RowCfg<T, 4, K>>(p, s);
-    if (p.c <= 64) return launch<RowCfg<T, 8, K>>(p, s);
-    if (p.c <= 128) return launch<RowCfg<T, 16, K>>(p, s);
-    if (p.c <= 256) return launch<RowCfg<T, 32, K>>(p, s);
-    if (p.c <= 512) return launch<RowCfg<T, 64, K>>(p, s);
-    if (p.c <= 1024) return launch<RowCfg<T, 64, 2 * K>>(p, s);
-    if (p.c <= 2048) return launch<RowCfg<T, 256, K>>(p, s);
-    if (p.c <= 4096) return launch<RowCfg<T, 256, 2 * K>>(p, s);
-    return launch<RowCfg<T, 512, 2 * K>>(p, s);
+    if (ODD && p.c < RowVec<T>::VEC) return launch<RowCfg<RowOne<T>, 8, 1, false>>(p, s);
+    if (p.c <= 16) return launch<RowCfg<RowVec<T>, 2, K, ODD>>(p, s);
+    if (p.c <= 32) return launch<RowCfg<RowVec<T>, 4, K, ODD>>(p, s);
+    if (p.c <= 64) return launch<RowCfg<RowVec<T>, 8, K, ODD>>(p, s);
+    if (p.c <= 128) return launch<RowCfg<RowVec<T>, 16, K, ODD>>(p, s);
+    if (p.c <= 256) return launch<RowCfg<RowVec<T>, 32, K, ODD>>(p, s);
+    if (p.c <= 512) return launch<RowCfg<RowVec<T>, 64, K, ODD>>(p, s);
+    if (p.c <= 1024) return launch<RowCfg<RowVec<T>, 64, 2 * K, ODD>>(p, s);
+    if (p.c <= 2048) return launch<RowCfg<RowVec<T>, 256, K, ODD>>(p, s);
+    if (p.c <= 4096) return launch<RowCfg<RowVec<T>, 256, 2 * K, ODD>>(p, s);
+    return launch<RowCfg<RowVec<T>, 512, 2 * K, ODD>>(p, s);
+}
+template <class T>
+int dispatch(const NormParams& p, hipStream_t s)
+{
+    return p.c % RowVec<T>::VEC ? dispatch<T, true>(p, s) : dispatch<T, false>(p, s);
 }
 
 }  // namespace

@@ -14,6 +14,8 @@
 // A work-group keeps its sums in registers (fp32), adds its row groups' through LDS and writes them to its own place of the
 // workspace; a second launch adds those in a fixed order.  No atomics: results repeat bit for bit.  Bound by HBM.
 #pragma once
+#include <atomic>
+
 #include "norm_residual.h"
 
 namespace srhip_norm {
@@ -48,15 +50,12 @@ __device__ __forceinline__ float gate_value(const NormBwdParams& p, const long l
 
 // Adds `acc` over the work-group's row groups, channel by channel, and hands (channel, sum) to `put`; every thread calls it.
 template <class C, class F>
-__device__ __forceinline__ void sum_row_groups(float* tile, const float* acc, const int c, F&& put)
+__device__ __forceinline__ void sum_row_groups(float* tile, const Lane<C>& l, const float* acc, const int c, F&& put)
 {
-    const int t = threadIdx.x % C::TPR;
     if constexpr (C::RPB == 1) {
 #pragma unroll
-        for (int j = 0; j < C::E; ++j) {
-            const int ch = (j / C::VEC * C::TPR + t) * C::VEC + j % C::VEC;
-            if (ch < c) put(ch, acc[j]);
-        }
+        for (int j = 0; j < C::E; ++j)
+            if (l.mine(j)) put(l.c0[j / C::VEC] + j % C::VEC, acc[j]);
     } else {
         // the groups of one wave by lane moves, the waves (or, of wider rows, the groups) through LDS
         constexpr int PARTS = C::TPR <= 64 ? C::THREADS / 64 : C::RPB;
@@ -65,10 +64,10 @@ __device__ __forceinline__ void sum_row_groups(float* tile, const float* acc, co
 #pragma unroll
         for (int j = 0; j < C::E; ++j) {
             const float v = C::TPR < 64 ? same_place_sum<C::TPR>(acc[j]) : acc[j];
-            if (C::TPR >= 64 || (threadIdx.x & 63) < C::TPR) tile[part * C::CMAX + (j / C::VEC * C::TPR + t) * C::VEC + j % C::VEC] = v;
+            if ((C::TPR >= 64 || (threadIdx.x & 63) < C::TPR) && l.mine(j)) tile[part * C::CMAX + l.c0[j / C::VEC] + j % C::VEC] = v;
         }
         __syncthreads();
-        for (int ch = threadIdx.x; ch < C::CMAX && ch < c; ch += C::THREADS) {
+        for (int ch = threadIdx.x; ch < c; ch += C::THREADS) {
             float s = tile[ch];
 #pragma unroll
             for (int k = 1; k < PARTS; ++k) s += tile[k * C::CMAX + ch];
@@ -81,36 +80,46 @@ constexpr int row_groups_tile() { return C::RPB == 1 ? C::THREADS / 64 : C::CMAX
 
 template <class C, bool CK>
 struct SavedRow {
-    using T = typename C::T;
     rows_u32x4 q[C::V];
-    // a row of a map, or of a checkpoint (words 0, 1: codes, word 3: scale byte)
-    __device__ __forceinline__ void load(const char* p, const unsigned char* scales, const long long row, const int c, const int groups, const int* c0, const int* nv, const bool whole)
+    // a lane's part of a row of a map, or of a checkpoint (words 0, 1: codes, word 3: scale byte)
+    __device__ __forceinline__ void load(const char* p, const unsigned char* scales, const long long pass, const NormBwdParams& np, const Lane<C>& l, const unsigned back, const unsigned back_rows)
     {
         if (CK && scales != nullptr) {
-            const unsigned char* codes = (const unsigned char*)p + row * c;
-            const unsigned char* sb = scales + row * groups;
+            const unsigned char* codes = (const unsigned char*)p + pass * np.c;
+            const unsigned char* sb = scales + pass * np.groups;
 #pragma unroll
             for (int v = 0; v < C::V; ++v) {
                 unsigned w[2] = {0u, 0u};
-                if (whole || nv[v] >= C::VEC) __builtin_memcpy(w, codes + c0[v], C::VEC);
-                else
-#pragma unroll
-                    for (int k = 0; k < C::VEC; ++k)
-                        if (k < nv[v]) w[k >> 2] |= (unsigned)codes[c0[v] + k] << (8 * (k & 3));
-                q[v][0] = w[0]; q[v][1] = w[1]; q[v][2] = 0u;
-                q[v][3] = whole || nv[v] > 0 ? sb[c0[v] / kCk8Group] : 0u;
+                __builtin_memcpy(w, codes + (size_t)(l.e[v] - back), C::VEC);
+                q[v][0] = w[0]; q[v][1] = w[1];
+                // (a vector that was moved to end with the row can lie across two groups: two scales)
+                const unsigned sr = (l.rg - back_rows) * np.groups;
+                q[v][3] = sb[(size_t)(sr + (unsigned)(l.c0[v] + C::VEC - 1) / kCk8Group)];
+                q[v][2] = C::ODD ? sb[(size_t)(sr + (unsigned)l.c0[v] / kCk8Group)] : 0u;
             }
         } else {
-            load_row<C>(p + row * c * RowVec<T>::SIZE, c0, nv, whole, q);
+            load_row<C>(p + pass * np.c * C::SIZE, l, back, q);
         }
     }
-    __device__ __forceinline__ void unpack(const unsigned char* scales, float* f) const
+    __device__ __forceinline__ void unpack(const unsigned char* scales, const Lane<C>& l, float* f) const
     {
         if (CK && scales != nullptr) {
 #pragma unroll
             for (int v = 0; v < C::V; ++v)
 #pragma unroll
-                for (int k = 0; k < C::VEC / 4; ++k) ck8_unpack4(q[v][k], ck8_scale(q[v][3]), f + v * C::VEC + 4 * k);
+                for (int k = 0; k < C::VEC; k += 4) {
+                    float g[4];
+                    ck8_unpack4(q[v][k / 4], ck8_scale(q[v][3]), g);
+                    if constexpr (C::ODD) {
+                        float a[4];
+                        ck8_unpack4(q[v][k / 4], ck8_scale(q[v][2]), a);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if ((l.c0[v] + k + i) / kCk8Group < (l.c0[v] + C::VEC - 1) / kCk8Group) g[i] = a[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4 && k + i < C::VEC; ++i) f[v * C::VEC + k + i] = g[i];
+                }
         } else {
             unpack_row<C>(q, f);
         }
@@ -122,44 +131,45 @@ template <class C, bool CK, bool MAPG>
 struct RawRow {
     SavedRow<C, CK> h, r;
     rows_u32x4 dr[C::V], dn[C::V], g[MAPG ? C::V : 1];
-    __device__ __forceinline__ void load(const NormBwdParams& p, const long long row, const int* c0, const int* nv, const bool whole)
+    // pass: first row; lanes behind the item's last row (`left` rows from the first on) work on it too and add nothing
+    __device__ __forceinline__ void load(const NormBwdParams& p, const long long pass, const long long left, const Lane<C>& l)
     {
-        const long long at = row * p.c * RowVec<typename C::T>::SIZE;
-        if (p.need_h) h.load(p.h, p.h_scales, row, p.c, p.groups, c0, nv, whole);
+        const unsigned back_rows = l.rg < left ? 0u : (unsigned)(l.rg - (int)(left - 1)), back = back_rows * p.c;
+        const long long at = pass * p.c * C::SIZE;
+        if (p.need_h) h.load(p.h, p.h_scales, pass, p, l, back, back_rows);
         if (p.pre) {
-            r.load(p.r, p.r_scales, row, p.c, p.groups, c0, nv, whole);
-            load_row<C>(p.dn + at, c0, nv, whole, dn);
+            r.load(p.r, p.r_scales, pass, p, l, back, back_rows);
+            load_row<C>(p.dn + at, l, back, dn);
         }
-        if (p.dr) load_row<C>(p.dr + at, c0, nv, whole, dr);
+        if (p.dr) load_row<C>(p.dr + at, l, back, dr);
         if constexpr (MAPG)
-            if (!p.gate_f32) load_row<C>(p.gate + at, c0, nv, whole, g);
+            if (!p.gate_f32) load_row<C>(p.gate + at, l, back, g);
     }
 };
 
+// Waves to a SIMD that the registers are to leave room for: four of the kernel that decodes short bf16 rows (it needs 137
+// registers left alone, and at 128, nine of them spilled, 64 channels of four crops take 587 us instead of 617), three with a
+// gate map (two crops: 469 us instead of 532; of fp32 maps 138 us instead of 79, they are left alone), else what the compiler
+// arrives at (the same on maps: 684 us for 681).
 template <class C, bool CK, bool MAPG>
-__global__ __launch_bounds__(C::THREADS) void norm_residual_bwd_kernel(const NormBwdParams p)
+constexpr int min_waves() { return C::SIZE == 2 && C::TPR <= 64 ? (MAPG ? 3 : CK ? 4 : 1) : 1; }
+
+template <class C, bool CK, bool MAPG>
+__global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG>())) void norm_residual_bwd_kernel(const NormBwdParams p)
 {
-    using T = typename C::T;
-    constexpr int SIZE = RowVec<T>::SIZE, VEC = C::VEC, E = C::E;
+    constexpr int SIZE = C::SIZE, VEC = C::VEC, E = C::E;
     __shared__ float scratch[row_sum_scratch<C>()];
     __shared__ float tile[row_groups_tile<C>()];
     RowSum<C> sum{scratch, 0};
-    const int t = threadIdx.x % C::TPR, rg = threadIdx.x / C::TPR;
-    const bool whole = p.c == C::CMAX;
-    int c0[C::V], nv[C::V];
-#pragma unroll
-    for (int v = 0; v < C::V; ++v) {
-        c0[v] = (v * C::TPR + t) * VEC;
-        nv[v] = p.c - c0[v];
-    }
+    const Lane<C> l(p.c);
     float wpre[E], sw[E];   // sw: scale (and, constant over an item, the gate) times the post norm's weight
     float sb[MAPG ? E : 1];
     float a_w[E], a_b[E], a1[E], a0[E];
-    load_params<C>(p.pre_w, c0, nv, 1.0f, wpre);
+    load_params<C>(p.pre_w, l, 1.0f, wpre);
     const float scale = p.scale_ptr ? *p.scale_ptr : p.scale;
     if constexpr (MAPG) {
-        load_params<C>(p.post_w, c0, nv, 1.0f, sw);
-        load_params<C>(p.post_b, c0, nv, 0.0f, sb);
+        load_params<C>(p.post_w, l, 1.0f, sw);
+        load_params<C>(p.post_b, l, 0.0f, sb);
 #pragma unroll
         for (int j = 0; j < E; ++j) { sw[j] *= scale; sb[j] *= scale; }
     }
@@ -171,18 +181,19 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_bwd_kernel(const Nor
         const long long r0 = s * p.rows_per_gate + (item - s * p.segs) * p.seg_rows;
         const long long end = (s + 1) * p.rows_per_gate;
         const long long r1 = r0 + p.seg_rows < end ? r0 + p.seg_rows : end;
-        // the next row's loads run ahead of the row at work, but where 16 elements a lane leave no registers for them
-        constexpr bool AHEAD = E <= 8;
+        // A work-group that holds one or two rows loads the next one ahead (16000 rows of 4096: 188 us, without 218), and so does
+        // one that decodes (64 channels of four crops from checkpoints: 621 us, without 673).  Otherwise, with many rows in
+        // flight, it gains nothing and costs registers; with 16 elements a lane there are none left for it.
+        constexpr bool AHEAD = (C::TPR > 64 || CK) && E <= 8;
         RawRow<C, CK, MAPG> next;
-        // lanes behind the item's last row work on it too and add nothing
-        if (AHEAD) next.load(p, r0 + rg < r1 ? r0 + rg : r1 - 1, c0, nv, whole);
+        if (AHEAD) next.load(p, r0, r1 - r0, l);
         if constexpr (!MAPG) {
-            load_params<C>(p.post_w, c0, nv, 1.0f, sw);
+            load_params<C>(p.post_w, l, 1.0f, sw);
 #pragma unroll
             for (int j = 0; j < E; ++j) sw[j] *= scale;
             if (p.gate_mode == SRHIP_GATE_ROWS) {
                 float g[E];
-                load_params<C>((const float*)p.gate + s * p.c, c0, nv, 0.0f, g);
+                load_params<C>((const float*)p.gate + s * p.c, l, 0.0f, g);
 #pragma unroll
                 for (int j = 0; j < E; ++j) sw[j] *= p.sigmoid ? sigmoid_f32(g[j]) : g[j];
             }
@@ -190,48 +201,45 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_bwd_kernel(const Nor
 #pragma unroll
         for (int j = 0; j < E; ++j) a1[j] = a0[j] = 0.0f;
         for (long long base = r0; base < r1; base += C::RPB) {
-            const bool live = base + rg < r1;
-            const long long row = live ? base + rg : r1 - 1;
-            const long long at = row * p.c * SIZE;
-            if (!AHEAD) next.load(p, row, c0, nv, whole);
+            const bool live = l.rg < r1 - base;
+            const long long at = base * p.c * SIZE;
+            if (!AHEAD) next.load(p, base, r1 - base, l);
             const RawRow<C, CK, MAPG> raw = next;
-            if (AHEAD && base + C::RPB < r1) next.load(p, base + C::RPB + rg < r1 ? base + C::RPB + rg : r1 - 1, c0, nv, whole);
+            if (AHEAD && base + C::RPB < r1) next.load(p, base + C::RPB, r1 - base - C::RPB, l);
 
             float r[E], h[E], d[E], rstd_r = 1.0f, rstd_h = 1.0f;
-            if (p.pre) raw.r.unpack(p.r_scales, r);
-            if (p.need_h) raw.h.unpack(p.h_scales, h);
-            normalise<C>(sum, p.pre, r, p.post, h, nv, p.layer, p.inv_c, p.eps, rstd_r, rstd_h);
+            if (p.pre) raw.r.unpack(p.r_scales, l, r);
+            if (p.need_h) raw.h.unpack(p.h_scales, l, h);
+            normalise<C>(sum, l, p.pre, r, p.post, h, p.layer, p.inv_c, p.eps, rstd_r, rstd_h);
 
             // ---- the norm behind the sum: dR
-#pragma unroll
-            for (int j = 0; j < E; ++j) d[j] = 0.0f;
             if (p.dr) unpack_row<C>(raw.dr, d);
+            else
+#pragma unroll
+                for (int j = 0; j < E; ++j) d[j] = 0.0f;
             if (p.pre) {
-                float q[E], m1 = 0.0f, m2 = 0.0f;
+                float q[E];
                 unpack_row<C>(raw.dn, q);
                 if (live)
 #pragma unroll
                     for (int j = 0; j < E; ++j) { a_w[j] += q[j] * r[j]; a_b[j] += q[j]; }
 #pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    q[j] *= wpre[j];
-                    m1 += q[j];
-                    m2 += q[j] * r[j];
-                }
+                for (int j = 0; j < E; ++j) q[j] *= wpre[j];
+                float m1 = 0.0f, m2 = lane_sum<C>(l, [&](int j) { return q[j] * r[j]; });
+                if (p.layer) m1 = lane_sum<C>(l, [&](int j) { return q[j]; });
                 sum.two(m1, m2);
-                m1 = p.layer ? -rstd_r * (m1 * p.inv_c) : 0.0f;
+                m1 = -rstd_r * (m1 * p.inv_c);
                 m2 = -rstd_r * (m2 * p.inv_c);
 #pragma unroll
                 for (int j = 0; j < E; ++j) d[j] = rstd_r * q[j] + (m2 * r[j] + (d[j] + m1));
-                zero_absent<C>(d, nv);
             }
-            if (live) store_row<C>(p.dx + at, c0, nv, whole, d);
+            if (live) store_row<C>(p.dx + at, l, d);
             if (!p.dh) continue;
 
             // ---- gate, scale and the norm in front of them: dh
             if constexpr (MAPG) {
                 float g[E];
-                if (p.gate_f32) load_gate_f32<C>(p.gate + row * p.c * 4, c0, nv, g);
+                if (p.gate_f32) load_gate_f32<C>(p.gate + base * p.c * 4, l, live ? 0u : (unsigned)((l.rg - (int)(r1 - base - 1)) * p.c), g);
                 else unpack_row<C>(raw.g, g);
                 if (p.sigmoid)
 #pragma unroll
@@ -247,9 +255,9 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_bwd_kernel(const Nor
                     if (p.gate_f32) {
 #pragma unroll
                         for (int j = 0; j < E; ++j)
-                            if (j % VEC < nv[j / VEC]) ((float*)p.dgate)[row * p.c + c0[j / VEC] + j % VEC] = dg[j];
+                            if (l.in[j / VEC]) ((float*)p.dgate + base * p.c)[l.e[j / VEC] + j % VEC] = dg[j];
                     } else {
-                        store_row<C>(p.dgate + at, c0, nv, whole, dg);
+                        store_row<C>(p.dgate + at, l, dg);
                     }
                 }
             }
@@ -259,29 +267,25 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_bwd_kernel(const Nor
 #pragma unroll
             for (int j = 0; j < E; ++j) d[j] *= sw[j];
             if (p.post) {
-                float m1 = 0.0f, m2 = 0.0f;
-#pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    m1 += d[j];
-                    m2 += d[j] * h[j];
-                }
+                float m1 = 0.0f, m2 = lane_sum<C>(l, [&](int j) { return d[j] * h[j]; });
+                if (p.layer) m1 = lane_sum<C>(l, [&](int j) { return d[j]; });
                 sum.two(m1, m2);
-                m1 = p.layer ? -rstd_h * (m1 * p.inv_c) : 0.0f;
+                m1 = -rstd_h * (m1 * p.inv_c);
                 m2 = -rstd_h * (m2 * p.inv_c);
 #pragma unroll
                 for (int j = 0; j < E; ++j) d[j] = rstd_h * d[j] + (m2 * h[j] + m1);
             }
-            if (live) store_row<C>(p.dh + at, c0, nv, whole, d);
+            if (live) store_row<C>(p.dh + at, l, d);
         }
         if (p.item_flush) {
             float* out = p.item_sums + item * 2 * p.c;
             float part = 0.0f;
-            sum_row_groups<C>(tile, a1, p.c, [&](const int ch, const float v) {
+            sum_row_groups<C>(tile, l, a1, p.c, [&](const int ch, const float v) {
                 float slope;
                 out[ch] = v;
                 if (p.dscale) part += v * gate_value(p, s, ch, slope) * (p.post_w ? p.post_w[ch] : 1.0f);
             });
-            sum_row_groups<C>(tile, a0, p.c, [&](const int ch, const float v) {
+            sum_row_groups<C>(tile, l, a0, p.c, [&](const int ch, const float v) {
                 float slope;
                 out[p.c + ch] = v;
                 if (p.dscale && p.post_b) part += v * gate_value(p, s, ch, slope) * p.post_b[ch];
@@ -300,8 +304,8 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_bwd_kernel(const Nor
     }
     if (p.pre) {
         float* out = p.wg_sums + (long long)blockIdx.x * 2 * p.c;
-        sum_row_groups<C>(tile, a_w, p.c, [&](const int ch, const float v) { out[ch] = v; });
-        sum_row_groups<C>(tile, a_b, p.c, [&](const int ch, const float v) { out[p.c + ch] = v; });
+        sum_row_groups<C>(tile, l, a_w, p.c, [&](const int ch, const float v) { out[ch] = v; });
+        sum_row_groups<C>(tile, l, a_b, p.c, [&](const int ch, const float v) { out[p.c + ch] = v; });
     }
 }
 
@@ -311,38 +315,64 @@ struct Plan {
     int segs, grid, rpb, threads;
 };
 
-template <class C, bool CK>
-void launch_rows(const NormBwdParams& p, const Plan& q, hipStream_t stream)
-{
-    if (p.gate_mode == SRHIP_GATE_MAP) hipLaunchKernelGGL((norm_residual_bwd_kernel<C, CK, true>), dim3(q.grid), dim3(C::THREADS), 0, stream, p);
-    else hipLaunchKernelGGL((norm_residual_bwd_kernel<C, CK, false>), dim3(q.grid), dim3(C::THREADS), 0, stream, p);
-}
-template <class C>
-int launch(const NormBwdParams& p, const Plan& q, hipStream_t stream)
-{
-    if (p.h_scales || p.r_scales) launch_rows<C, true>(p, q, stream);
-    else launch_rows<C, false>(p, q, stream);
-    return srhip_check_launch("norm_residual_bwd_kernel");
-}
-
-template <class T>
-int dispatch(const NormBwdParams& p, const Plan& q, hipStream_t s)
+// Calls f with the configuration of a row of c channels: the narrowest group of lanes that holds it.
+template <class T, bool ODD, class F>
+int with_rows(const int c, F&& f)
 {
     constexpr int K = 8 / RowVec<T>::VEC;   // vectors for 8 channels
-    if (p.c <= 16) return launch<RowCfg<T, 2, K>>(p, q, s);
-    if (p.c <= 32) return launch<RowCfg<T, 4, K>>(p, q, s);
-    if (p.c <= 64) return launch<RowCfg<T, 8, K>>(p, q, s);
-    if (p.c <= 128) return launch<RowCfg<T, 16, K>>(p, q, s);
-    if (p.c <= 256) return launch<RowCfg<T, 32, K>>(p, q, s);
-    if (p.c <= 512) return launch<RowCfg<T, 64, K>>(p, q, s);
-    if (p.c <= 1024) return launch<RowCfg<T, 128, K>>(p, q, s);
-    if (p.c <= 2048) return launch<RowCfg<T, 256, K>>(p, q, s);
-    if (p.c <= 4096) return launch<RowCfg<T, 512, K>>(p, q, s);
-    return launch<RowCfg<T, 512, 2 * K>>(p, q, s);
+    if (ODD && c < RowVec<T>::VEC) return f(RowCfg<RowOne<T>, 8, 1, false>{});
+    if (c <= 16) return f(RowCfg<RowVec<T>, 2, K, ODD>{});
+    if (c <= 32) return f(RowCfg<RowVec<T>, 4, K, ODD>{});
+    if (c <= 64) return f(RowCfg<RowVec<T>, 8, K, ODD>{});
+    if (c <= 128) return f(RowCfg<RowVec<T>, 16, K, ODD>{});
+    if (c <= 256) return f(RowCfg<RowVec<T>, 32, K, ODD>{});
+    if (c <= 512) return f(RowCfg<RowVec<T>, 64, K, ODD>{});
+    if (c <= 1024) return f(RowCfg<RowVec<T>, 128, K, ODD>{});
+    if (c <= 2048) return f(RowCfg<RowVec<T>, 256, K, ODD>{});
+    if (c <= 4096) return f(RowCfg<RowVec<T>, 512, K, ODD>{});
+    return f(RowCfg<RowVec<T>, 512, 2 * K, ODD>{});
 }
 
-// the two map types are compiled side by side
-int rows_bf16(const NormBwdParams& p, const Plan& q, hipStream_t stream);
-int rows_f32(const NormBwdParams& p, const Plan& q, hipStream_t stream);
+// How many work-groups of the call's kernel a CU holds, and their shape; asked of the runtime once per kernel and device.
+template <class C, bool CK, bool MAPG>
+void shape_of(Plan& q)
+{
+    static std::atomic<int> fit[kSrhipMaxDevices];
+    const int dev = srhip_current_device();
+    int n = fit[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, norm_residual_bwd_kernel<C, CK, MAPG>, C::THREADS, 0) != hipSuccess || n < 1) n = 1;
+        fit[dev].store(n, std::memory_order_relaxed);
+    }
+    q.grid = n;
+    q.rpb = C::RPB;
+    q.threads = C::THREADS;
+}
+template <class C, bool CK, bool MAPG>
+int shape_or_launch(const NormBwdParams* p, Plan& q, hipStream_t stream)
+{
+    if (p == nullptr) {
+        shape_of<C, CK, MAPG>(q);
+        return SRHIP_OK;
+    }
+    hipLaunchKernelGGL((norm_residual_bwd_kernel<C, CK, MAPG>), dim3(q.grid), dim3(C::THREADS), 0, stream, *p);
+    return srhip_check_launch("norm_residual_bwd_kernel");
+}
+template <class T, bool ODD>
+int rows_of(const int c, const bool ck, const bool mapg, const NormBwdParams* p, Plan& q, hipStream_t stream)
+{
+    return with_rows<T, ODD>(c, [&](auto cfg) {
+        using C = decltype(cfg);
+        if (ck) return mapg ? shape_or_launch<C, true, true>(p, q, stream) : shape_or_launch<C, true, false>(p, q, stream);
+        return mapg ? shape_or_launch<C, false, true>(p, q, stream) : shape_or_launch<C, false, false>(p, q, stream);
+    });
+}
+
+// Compiled side by side, by map type and whether channels come in whole vectors.  p null: the kernel's shape into q (grid =
+// work-groups to a CU); otherwise its launch as q says.
+int rows_bf16(int c, bool ck, bool mapg, const NormBwdParams* p, Plan& q, hipStream_t stream);
+int rows_bf16_odd(int c, bool ck, bool mapg, const NormBwdParams* p, Plan& q, hipStream_t stream);
+int rows_f32(int c, bool ck, bool mapg, const NormBwdParams* p, Plan& q, hipStream_t stream);
+int rows_f32_odd(int c, bool ck, bool mapg, const NormBwdParams* p, Plan& q, hipStream_t stream);
 
 }  // namespace srhip_norm

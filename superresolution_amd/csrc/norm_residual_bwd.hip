@@ -68,17 +68,21 @@ __global__ __launch_bounds__(1024) void norm_residual_bwd_sums_kernel(const Norm
     }
 }
 
-// Items and work-groups: a function of the shape alone (and of the device's CUs), so that the
-// workspace can be sized before the call.
+int rows(const srhip_norm_residual_bwd_args* a, const NormBwdParams* p, Plan& q, hipStream_t stream)
+{
+    const bool ck = a->h_scales || a->r_scales, mapg = a->gate_mode == SRHIP_GATE_MAP;
+    if (a->dtype == SRHIP_DT_BF16) return (a->c % 8 ? rows_bf16_odd : rows_bf16)(a->c, ck, mapg, p, q, stream);
+    return (a->c % 4 ? rows_f32_odd : rows_f32)(a->c, ck, mapg, p, q, stream);
+}
+
+// Items and work-groups: a function of the shapes and types alone (and of the device), so that the workspace can be sized before
+// the call.
 Plan plan_of(const srhip_norm_residual_bwd_args* a)
 {
     Plan q;
-    const int tpr = a->c <= 16 ? 2 : a->c <= 32 ? 4 : a->c <= 64 ? 8 : a->c <= 128 ? 16 : a->c <= 256 ? 32 : a->c <= 512 ? 64
-                    : a->c <= 1024 ? 128 : a->c <= 2048 ? 256 : 512;
-    q.threads = tpr <= 256 ? 256 : tpr;
-    q.rpb = q.threads / tpr;
+    rows(a, nullptr, q, nullptr);
     const long long passes = (a->rows + q.rpb - 1) / q.rpb;
-    const long long cus = srhip_num_cus(), resident = cus * (768 / q.threads > 0 ? 768 / q.threads : 1);
+    const long long cus = srhip_num_cus(), resident = cus * q.grid;
     // A work-group's sums (4 c floats written, and read again) weigh as much as one or two of its rows: eight passes to a
     // work-group at least, once every CU has one.
     long long grid = passes / 8;
@@ -132,7 +136,7 @@ SRHIP_API int srhip_norm_residual_bwd(const srhip_norm_residual_bwd_args* a, voi
     const int need_h = a->dh && (a->post || a->gate_mode != SRHIP_GATE_NONE || a->dscale);
     SRHIP_REQUIRE(!need_h || a->h, "norm_residual_bwd: null branch");
     SRHIP_REQUIRE(a->workspace, "norm_residual_bwd: null workspace");
-    const Plan q = plan_of(a);
+    Plan q = plan_of(a);
     NormBwdParams p;
     p.h = (const char*)a->h; p.r = (const char*)a->r; p.dr = (const char*)a->dr; p.dn = (const char*)a->dn; p.gate = (const char*)a->gate;
     p.h_scales = (const unsigned char*)a->h_scales; p.r_scales = (const unsigned char*)a->r_scales;
@@ -157,7 +161,7 @@ SRHIP_API int srhip_norm_residual_bwd(const srhip_norm_residual_bwd_args* a, voi
     const int cblocks = srhip_div_up(p.c, 64);
     const long long blocks = (5 + (p.gate_mode == SRHIP_GATE_ROWS ? gates : 0)) * cblocks;
     SRHIP_REQUIRE(blocks < (1ll << 31), "norm_residual_bwd: too many gates");
-    const int launched = a->dtype == SRHIP_DT_BF16 ? rows_bf16(p, q, s) : rows_f32(p, q, s);
+    const int launched = rows(a, &p, q, s);
     if (launched != SRHIP_OK || (!p.pre && !p.item_flush)) return launched;
     hipLaunchKernelGGL(norm_residual_bwd_sums_kernel, dim3((unsigned)blocks), dim3(1024), 0, s, p, q.grid, cblocks);
     return srhip_check_launch("norm_residual_bwd_sums_kernel");

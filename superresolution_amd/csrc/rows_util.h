@@ -10,10 +10,21 @@ typedef __attribute__((ext_vector_type(2))) unsigned rows_u32x2;
 
 // ---- one vector of 16 bytes = VEC elements.  Rows of odd channel counts start at any element: gfx950 reads and writes
 // global memory at any alignment with one instruction, so the same 16-byte access serves every row.
+__device__ __forceinline__ rows_u32x4 load16(const char* p)
+{
+    rows_u32x4 q;
+    __builtin_memcpy(&q, p, 16);
+    return q;
+}
+__device__ __forceinline__ void store16(char* p, const rows_u32x4 q) { __builtin_memcpy(p, &q, 16); }
+
 template <class T>
 struct RowVec;
 template <>
 struct RowVec<__bf16> {
+    using T = __bf16;
+    __device__ static __forceinline__ rows_u32x4 load(const char* p) { return load16(p); }
+    __device__ static __forceinline__ void store(char* p, const rows_u32x4 q) { store16(p, q); }
     static constexpr int VEC = 8, SIZE = 2;
     __device__ static __forceinline__ void unpack(const rows_u32x4 q, float* f)
     {
@@ -30,6 +41,9 @@ struct RowVec<__bf16> {
 };
 template <>
 struct RowVec<float> {
+    using T = float;
+    __device__ static __forceinline__ rows_u32x4 load(const char* p) { return load16(p); }
+    __device__ static __forceinline__ void store(char* p, const rows_u32x4 q) { store16(p, q); }
     static constexpr int VEC = 4, SIZE = 4;
     __device__ static __forceinline__ void unpack(const rows_u32x4 q, float* f)
     {
@@ -45,13 +59,32 @@ struct RowVec<float> {
     }
 };
 
-__device__ __forceinline__ rows_u32x4 load16(const char* p)
-{
-    rows_u32x4 q;
-    __builtin_memcpy(&q, p, 16);
-    return q;
-}
-__device__ __forceinline__ void store16(char* p, const rows_u32x4 q) { __builtin_memcpy(p, &q, 16); }
+// One element instead of a vector, for rows that are shorter than one.
+template <class T_>
+struct RowOne {
+    using T = T_;
+    static constexpr int VEC = 1, SIZE = RowVec<T>::SIZE;
+    __device__ static __forceinline__ rows_u32x4 load(const char* p)
+    {
+        rows_u32x4 q = {0u, 0u, 0u, 0u};
+        unsigned w = 0u;
+        __builtin_memcpy(&w, p, SIZE);
+        q[0] = w;
+        return q;
+    }
+    __device__ static __forceinline__ void store(char* p, const rows_u32x4 q)
+    {
+        const unsigned w = q[0];
+        __builtin_memcpy(p, &w, SIZE);
+    }
+    __device__ static __forceinline__ void unpack(const rows_u32x4 q, float* f) { f[0] = SIZE == 2 ? bf16_lo(q[0]) : __uint_as_float(q[0]); }
+    __device__ static __forceinline__ rows_u32x4 pack(const float* f)
+    {
+        rows_u32x4 q = {0u, 0u, 0u, 0u};
+        q[0] = SIZE == 2 ? f32_to_bf16_bits(f[0]) : __float_as_uint(f[0]);
+        return q;
+    }
+};
 
 // The first `nv` elements (of SIZE bytes) of a vector whose 16 bytes reach past the end of the row; the others are 0.
 template <int SIZE>
@@ -160,12 +193,18 @@ constexpr int kCk8Lowest = 10;
 constexpr unsigned kCk8Largest = 0x7f600000u;
 
 __device__ __forceinline__ float ck8_scale(const unsigned s) { return __uint_as_float(s << 23); }
-// values of the 4 codes in w
+// values of the 4 codes in w (one instruction decodes and scales two: exact, the scale is a power of two)
 __device__ __forceinline__ void ck8_unpack4(const unsigned w, const float scale, float* f)
 {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
-    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-    f[0] = lo[0] * scale; f[1] = lo[1] * scale; f[2] = hi[0] * scale; f[3] = hi[1] * scale;
+    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, false);
+    const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, true);
+    f[0] = lo[0]; f[1] = lo[1]; f[2] = hi[0]; f[3] = hi[1];
+}
+// ... as bf16 pairs, exact as well
+__device__ __forceinline__ void ck8_unpack4_bf16(const unsigned w, const float scale, unsigned& lo, unsigned& hi)
+{
+    lo = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+    hi = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true));
 }
 
 }  // namespace

@@ -60,6 +60,17 @@ def test_every_bf16_number_beside_a_large_one(F):
         _check_pack(F, torch.stack([x, torch.full_like(x, 1.5 * 2.0 ** k)], -1))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_every_code_with_every_scale(F, dtype):
+    """What a checkpoint can hold, all of it: 256 codes times the scale bytes 10 .. 246, exact."""
+    s = torch.arange(10, 247, dtype=torch.uint8)
+    codes = torch.arange(256, dtype=torch.uint8).view(1, 8, 32).expand(237, 8, 32).reshape(237, 256).contiguous()
+    scales = s[:, None].expand(237, 8).contiguous()
+    y = F.checkpoint8_restore(F.Checkpoint8(codes.cuda().view(torch.float8_e4m3fn), scales.cuda(), dtype)).cpu()
+    want = orc.decode(codes, scales)
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(y.double().nan_to_num(), want.nan_to_num())
+
+
 def test_error_of_a_checkpoint(F):
     """Half a step of 3 mantissa bits (2^-4 of the value), or less than the smallest code where that is larger."""
     g = torch.Generator().manual_seed(2)
