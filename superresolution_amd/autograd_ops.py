@@ -297,7 +297,7 @@ def _auto_wgrad(srcs, dzs: Tensor, w: Tensor):
     the MFMA weight-gradient kernel per (<= 64 input, <= 64 output) channel slice pair (a GEMM over a million pixels with a
     160 x 160 output is a shape the GEMM library serves three times slower than that)."""
     cout, cin, k, _ = w.shape
-    return F_.conv_wgrad(srcs, dzs, cin, cout, k)
+    return F_._conv_wgrad(srcs, dzs, cin, cout, k)
 
 
 def _dgrad_rows(dzs: Tensor, w: Tensor, row0: int, rows: int, mask: Tensor = None) -> Tensor:

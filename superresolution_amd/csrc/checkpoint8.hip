@@ -20,11 +20,12 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// ---- encode one chunk of 8 channels held by a lane; the four lanes of a quad hold the 32 channels of a group
+// ---- encode one chunk of 8 channels held by a lane; LANES lanes side by side (4: 32 channels) hold a group
 struct Encoded {
     rows_u32x2 codes;
     unsigned scale;
 };
+template <int LANES>
 __device__ __forceinline__ Encoded ck8_encode(float* f)
 {
     float a = 0.0f;
@@ -40,7 +41,7 @@ __device__ __forceinline__ Encoded ck8_encode(float* f)
             a = fmaxf(a, fabsf(f[j]));
         }
     }
-    a = lanes_max<4>(a);
+    a = lanes_max<LANES>(a);
     // a mantissa above 1.75 carries into the exponent field
     int e = (int)((__float_as_uint(a) + 0x1fffffu) >> 23) - 8;
     e = e < kCk8Lowest ? kCk8Lowest : e;
@@ -96,7 +97,8 @@ __device__ __forceinline__ void store_codes8(unsigned char* p, const rows_u32x2 
             if (j < nv) p[j] = (unsigned char)(q[j >> 2] >> (8 * (j & 3)));
 }
 
-// Where a lane's chunk lies.  A quad of lanes serves one (row, group of 32 channels) unit.
+// Where a lane's chunk lies.  LANES lanes serve one (row, group of 32 channels) unit: four, or, of maps that have no more than
+// 16 or 8 channels, two or one.
 struct Chunk {
     long long at;      // first element in the map
     long long unit;    // place of the group's scale
@@ -114,18 +116,18 @@ __device__ __forceinline__ Chunk chunk_of(const long long unit, const int q, con
     return k;
 }
 
-template <class T>
+template <class T, int LANES>
 __global__ __launch_bounds__(kThreads) void checkpoint8_pack_kernel(const char* __restrict__ x, unsigned char* __restrict__ codes,
                                                                     unsigned char* __restrict__ scales, const long long units,
                                                                     const int c, const int groups)
 {
-    const int q = threadIdx.x & 3;
-    const long long unit = (long long)blockIdx.x * (kThreads / 4) + (threadIdx.x >> 2);
-    if (unit >= units) return;   // whole quads
+    const int q = threadIdx.x % LANES;
+    const long long unit = (long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+    if (unit >= units) return;   // all lanes of a unit
     const Chunk k = chunk_of(unit, q, c, groups);
     float f[8];
     load8<T>(x + k.at * RowVec<T>::SIZE, k.nv, f);
-    const Encoded r = ck8_encode(f);
+    const Encoded r = ck8_encode<LANES>(f);
     store_codes8(codes + k.at, r.codes, k.nv);
     if (q == 0) scales[unit] = (unsigned char)r.scale;
 }
@@ -151,7 +153,7 @@ __global__ __launch_bounds__(kThreads) void checkpoint8_pack_signbits_kernel(con
             RowVec<__bf16>::unpack(load16(x + chunk * 16), f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) word |= f[j] > 0.0f ? 1u << (8 * k + j) : 0u;
-            const Encoded r = ck8_encode(f);
+            const Encoded r = ck8_encode<4>(f);
             *(rows_u32x2*)(codes + chunk * 8) = r.codes;
             if ((lane & 3) == 0) scales[chunk >> 2] = (unsigned char)r.scale;
         }
@@ -159,13 +161,13 @@ __global__ __launch_bounds__(kThreads) void checkpoint8_pack_signbits_kernel(con
     bits[wv * 64 + lane] = word;
 }
 
-template <class T>
+template <class T, int LANES>
 __global__ __launch_bounds__(kThreads) void checkpoint8_restore_kernel(const unsigned char* __restrict__ codes,
                                                                        const unsigned char* __restrict__ scales, char* __restrict__ y,
                                                                        const long long units, const int c, const int groups)
 {
-    const int q = threadIdx.x & 3;
-    const long long unit = (long long)blockIdx.x * (kThreads / 4) + (threadIdx.x >> 2);
+    const int q = threadIdx.x % LANES;
+    const long long unit = (long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
     if (unit >= units) return;
     const Chunk k = chunk_of(unit, q, c, groups);
     const rows_u32x2 w = load_codes8(codes + k.at, k.nv);
@@ -196,6 +198,50 @@ __global__ __launch_bounds__(kThreads) void relu_mask_checkpoint8_kernel(const c
 // rows of one launch: units (rows times groups) stay below 2^31
 long long slab_rows(const int groups) { return ((1ll << 31) - 1) / groups; }
 
+template <class T, int LANES>
+int pack_slab(const char* x, unsigned char* codes, unsigned char* scales, const long long units, const int c, const int groups, hipStream_t s)
+{
+    hipLaunchKernelGGL((checkpoint8_pack_kernel<T, LANES>), dim3((unsigned)((units + kThreads / LANES - 1) / (kThreads / LANES))), dim3(kThreads), 0, s,
+                       x, codes, scales, units, c, groups);
+    return srhip_check_launch("checkpoint8_pack_kernel");
+}
+template <class T, int LANES>
+int restore_slab(const unsigned char* codes, const unsigned char* scales, char* y, const long long units, const int c, const int groups, hipStream_t s)
+{
+    hipLaunchKernelGGL((checkpoint8_restore_kernel<T, LANES>), dim3((unsigned)((units + kThreads / LANES - 1) / (kThreads / LANES))), dim3(kThreads), 0, s,
+                       codes, scales, y, units, c, groups);
+    return srhip_check_launch("checkpoint8_restore_kernel");
+}
+// (Two 540 x 959 maps of ten fp32 channels: with four lanes to a row 17 us, with two 13.6.)
+template <class T>
+int pack_rows(const char* x, unsigned char* codes, unsigned char* scales, const long long rows, const int c, hipStream_t s)
+{
+    const int groups = srhip_div_up(c, kCk8Group);
+    for (long long r = 0; r < rows; r += slab_rows(groups)) {
+        const long long units = (rows - r < slab_rows(groups) ? rows - r : slab_rows(groups)) * groups;
+        const char* xs = x + r * c * RowVec<T>::SIZE;
+        unsigned char *cs = codes + r * c, *ss = scales + r * groups;
+        const int rc = c <= 8 ? pack_slab<T, 1>(xs, cs, ss, units, c, groups, s) : c <= 16 ? pack_slab<T, 2>(xs, cs, ss, units, c, groups, s)
+                                                                                           : pack_slab<T, 4>(xs, cs, ss, units, c, groups, s);
+        if (rc != SRHIP_OK) return rc;
+    }
+    return SRHIP_OK;
+}
+template <class T>
+int restore_rows(const unsigned char* codes, const unsigned char* scales, char* y, const long long rows, const int c, hipStream_t s)
+{
+    const int groups = srhip_div_up(c, kCk8Group);
+    for (long long r = 0; r < rows; r += slab_rows(groups)) {
+        const long long units = (rows - r < slab_rows(groups) ? rows - r : slab_rows(groups)) * groups;
+        const unsigned char *cs = codes + r * c, *ss = scales + r * groups;
+        char* ys = y + r * c * RowVec<T>::SIZE;
+        const int rc = c <= 8 ? restore_slab<T, 1>(cs, ss, ys, units, c, groups, s) : c <= 16 ? restore_slab<T, 2>(cs, ss, ys, units, c, groups, s)
+                                                                                              : restore_slab<T, 4>(cs, ss, ys, units, c, groups, s);
+        if (rc != SRHIP_OK) return rc;
+    }
+    return SRHIP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -206,22 +252,8 @@ SRHIP_API int srhip_checkpoint8_pack(const void* x, int dtype, void* codes, void
     SRHIP_REQUIRE(dtype == SRHIP_DT_BF16 || dtype == SRHIP_DT_F32, "checkpoint8_pack: unknown type %d", dtype);
     if (rows == 0) return SRHIP_OK;
     SRHIP_REQUIRE(x && codes && scales, "checkpoint8_pack: null pointer");
-    const int groups = srhip_div_up(c, kCk8Group);
-    const int size = dtype == SRHIP_DT_BF16 ? 2 : 4;
-    for (long long r = 0; r < rows; r += slab_rows(groups)) {
-        const long long units = (rows - r < slab_rows(groups) ? rows - r : slab_rows(groups)) * groups;
-        const dim3 grid((unsigned)((units + kThreads / 4 - 1) / (kThreads / 4)));
-        const char* xs = (const char*)x + r * c * size;
-        unsigned char* cs = (unsigned char*)codes + r * c;
-        unsigned char* ss = (unsigned char*)scales + r * groups;
-        if (dtype == SRHIP_DT_BF16)
-            hipLaunchKernelGGL(checkpoint8_pack_kernel<__bf16>, grid, dim3(kThreads), 0, (hipStream_t)stream, xs, cs, ss, units, c, groups);
-        else
-            hipLaunchKernelGGL(checkpoint8_pack_kernel<float>, grid, dim3(kThreads), 0, (hipStream_t)stream, xs, cs, ss, units, c, groups);
-        const int rc = srhip_check_launch("checkpoint8_pack_kernel");
-        if (rc != SRHIP_OK) return rc;
-    }
-    return SRHIP_OK;
+    return (dtype == SRHIP_DT_BF16 ? pack_rows<__bf16> : pack_rows<float>)((const char*)x, (unsigned char*)codes, (unsigned char*)scales, rows, c,
+                                                                            (hipStream_t)stream);
 }
 
 SRHIP_API int srhip_checkpoint8_pack_signbits(const void* x, void* codes, void* scales, void* signbits, int n, int h, int w, void* stream)
@@ -246,22 +278,8 @@ SRHIP_API int srhip_checkpoint8_restore(const void* codes, const void* scales, v
     SRHIP_REQUIRE(dtype == SRHIP_DT_BF16 || dtype == SRHIP_DT_F32, "checkpoint8_restore: unknown type %d", dtype);
     if (rows == 0) return SRHIP_OK;
     SRHIP_REQUIRE(codes && scales && y, "checkpoint8_restore: null pointer");
-    const int groups = srhip_div_up(c, kCk8Group);
-    const int size = dtype == SRHIP_DT_BF16 ? 2 : 4;
-    for (long long r = 0; r < rows; r += slab_rows(groups)) {
-        const long long units = (rows - r < slab_rows(groups) ? rows - r : slab_rows(groups)) * groups;
-        const dim3 grid((unsigned)((units + kThreads / 4 - 1) / (kThreads / 4)));
-        const unsigned char* cs = (const unsigned char*)codes + r * c;
-        const unsigned char* ss = (const unsigned char*)scales + r * groups;
-        char* ys = (char*)y + r * c * size;
-        if (dtype == SRHIP_DT_BF16)
-            hipLaunchKernelGGL(checkpoint8_restore_kernel<__bf16>, grid, dim3(kThreads), 0, (hipStream_t)stream, cs, ss, ys, units, c, groups);
-        else
-            hipLaunchKernelGGL(checkpoint8_restore_kernel<float>, grid, dim3(kThreads), 0, (hipStream_t)stream, cs, ss, ys, units, c, groups);
-        const int rc = srhip_check_launch("checkpoint8_restore_kernel");
-        if (rc != SRHIP_OK) return rc;
-    }
-    return SRHIP_OK;
+    return (dtype == SRHIP_DT_BF16 ? restore_rows<__bf16> : restore_rows<float>)((const unsigned char*)codes, (const unsigned char*)scales, (char*)y,
+                                                                                  rows, c, (hipStream_t)stream);
 }
 
 SRHIP_API int srhip_relu_mask_checkpoint8(const void* dy, const void* codes, void* out, size_t n, void* stream)

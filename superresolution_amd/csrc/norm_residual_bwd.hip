@@ -6,58 +6,80 @@ using namespace srhip_norm;
 
 namespace {
 
-// Adds the sums of work-groups and items: 64 columns to a block, 16 thread groups taking every 16th sum, then theirs in
-// order.  Block b: section b / cblocks (0, 1: dw_pre, db_pre; 2, 3: dw_post, db_post; 4: ds; 5 + i: gate i) of 64 channels.
-__global__ __launch_bounds__(1024) void norm_residual_bwd_sums_kernel(const NormBwdParams p, const int nwg, const int cblocks)
+// Adds the sums of work-groups and items: 32 columns to a block, 32 thread groups taking every 32nd sum, then theirs in
+// order.  Block b: section b / cblocks (0, 1: dw_pre, db_pre; 2, 3: dw_post, db_post; 4: ds; 5 + i: gate i) of 32 channels.
+// A chain of dependent-looking loads is what bounds it: a thousand sums in 32 steps of eight loads each (4.6 MB; 64 columns and
+// 16 groups, with a division by the items of a gate in every step, took 34 us for 64 channels, this 5).
+constexpr int kCols = 32, kParts = 32;
+__global__ __launch_bounds__(kCols * kParts) void norm_residual_bwd_sums_kernel(const NormBwdParams p, const int nwg, const int cblocks)
 {
-    __shared__ float red[2][16][64];
-    const int col = threadIdx.x & 63, part = threadIdx.x >> 6;
+    __shared__ float red[2][kParts][kCols];
+    const int col = threadIdx.x % kCols, part = threadIdx.x / kCols;
     const int section = (int)(blockIdx.x / (unsigned)cblocks);
-    const int ch = (int)(blockIdx.x % (unsigned)cblocks) * 64 + col;
+    const int ch = (int)(blockIdx.x % (unsigned)cblocks) * kCols + col;
     const bool in = ch < p.c;
     const float scale = p.scale_ptr ? *p.scale_ptr : p.scale;
     float a = 0.0f, b = 0.0f;
     if (section < 2) {
         float* dst = section == 0 ? p.dpre_w : p.dpre_b;
         if (dst == nullptr) return;   // uniform over the block, as all that follow
-        if (in)
-#pragma unroll 4
-            for (long long k = part; k < nwg; k += 16) a += p.wg_sums[(k * 2 + section) * p.c + ch];
+        if (in) {
+            const float* src = p.wg_sums + section * p.c + ch;
+#pragma unroll 8
+            for (int k = part; k < nwg; k += kParts) a += src[2ll * k * p.c];
+        }
     } else if (section < 4) {
         float* dst = section == 2 ? p.dpost_w : p.dpost_b;
         if (dst == nullptr) return;
-        if (in)
-#pragma unroll 4
-            for (long long k = part; k < p.items; k += 16) {
+        if (in) {
+            const float* src = p.item_sums + (section - 2) * p.c + ch;
+            if (p.gate_mode == SRHIP_GATE_ROWS && p.items > p.segs) {
+                // several gates: each item's sum times its gate
+                long long s = part / p.segs;
+                int rem = part % p.segs;
+                const int s_step = kParts / p.segs, r_step = kParts % p.segs;
+#pragma unroll 8
+                for (long long k = part; k < p.items; k += kParts) {
+                    float slope;
+                    a += gate_value(p, s, ch, slope) * src[2 * k * p.c];
+                    s += s_step;
+                    rem += r_step;
+                    if (rem >= p.segs) { rem -= p.segs; ++s; }
+                }
+            } else {
+#pragma unroll 8
+                for (long long k = part; k < p.items; k += kParts) a += src[2 * k * p.c];
                 float slope;
-                a += gate_value(p, k / p.segs, ch, slope) * p.item_sums[(k * 2 + section - 2) * p.c + ch];
+                a *= gate_value(p, 0, ch, slope);
             }
+        }
     } else if (section == 4) {
         if (p.dscale == nullptr || blockIdx.x % (unsigned)cblocks != 0) return;
-        for (long long k = threadIdx.x; k < p.items; k += 1024) a += p.item_scale[k];
+#pragma unroll 4
+        for (long long k = threadIdx.x; k < p.items; k += kCols * kParts) a += p.item_scale[k];
     } else {
         const long long s = section - 5;
-        if (in)
-#pragma unroll 4
-            for (long long k = part; k < p.segs; k += 16) {
-                a += p.item_sums[(s * p.segs + k) * 2 * p.c + ch];
-                b += p.item_sums[((s * p.segs + k) * 2 + 1) * p.c + ch];
+        if (in) {
+            const float* src = p.item_sums + s * p.segs * 2 * p.c + ch;
+#pragma unroll 8
+            for (int k = part; k < p.segs; k += kParts) {
+                a += src[2ll * k * p.c];
+                b += src[(2ll * k + 1) * p.c];
             }
+        }
     }
     red[0][part][col] = a;
     red[1][part][col] = b;
     __syncthreads();
-    if (section == 4) {
-        if (part != 0) return;
+    if (part != 0) return;
 #pragma unroll
-        for (int k = 1; k < 16; ++k) a += red[0][k][col];
-        a = lanes_sum<64>(a);
+    for (int k = 1; k < kParts; ++k) { a += red[0][k][col]; b += red[1][k][col]; }
+    if (section == 4) {
+        a = lanes_sum<kCols>(a);
         if (col == 0) *p.dscale = a;
         return;
     }
-    if (part != 0 || !in) return;
-#pragma unroll
-    for (int k = 1; k < 16; ++k) { a += red[0][k][col]; b += red[1][k][col]; }
+    if (!in) return;
     if (section < 2) (section == 0 ? p.dpre_w : p.dpre_b)[ch] = a;
     else if (section < 4) (section == 2 ? p.dpost_w : p.dpost_b)[ch] = scale * a;
     else {
@@ -158,12 +180,12 @@ SRHIP_API int srhip_norm_residual_bwd(const srhip_norm_residual_bwd_args* a, voi
     p.scale = a->scale; p.eps = a->eps; p.inv_c = 1.0f / (float)a->c;
     const long long gates = a->rows / p.rows_per_gate;
     const hipStream_t s = (hipStream_t)stream;
-    const int cblocks = srhip_div_up(p.c, 64);
+    const int cblocks = srhip_div_up(p.c, kCols);
     const long long blocks = (5 + (p.gate_mode == SRHIP_GATE_ROWS ? gates : 0)) * cblocks;
     SRHIP_REQUIRE(blocks < (1ll << 31), "norm_residual_bwd: too many gates");
     const int launched = rows(a, &p, q, s);
     if (launched != SRHIP_OK || (!p.pre && !p.item_flush)) return launched;
-    hipLaunchKernelGGL(norm_residual_bwd_sums_kernel, dim3((unsigned)blocks), dim3(1024), 0, s, p, q.grid, cblocks);
+    hipLaunchKernelGGL(norm_residual_bwd_sums_kernel, dim3((unsigned)blocks), dim3(kCols * kParts), 0, s, p, q.grid, cblocks);
     return srhip_check_launch("norm_residual_bwd_sums_kernel");
 }
 

@@ -341,20 +341,20 @@ def conv3x3_wgrad_multi(jobs, dw: torch.Tensor, db: Optional[torch.Tensor], ci_t
     shape = None
     w_i = dw.shape[1]
     held = isinstance(jobs[0][0], Checkpoint8)
-    scales, alive = (ctypes.c_void_p * len(jobs))(), []
+    scales = (ctypes.c_void_p * len(jobs))()
+    checked = {}   # tensors that passed (several jobs share a map), as contiguous copies that live until the launch is queued
     for j, (x, xo, ci_real, ci_off, dz, zo, co_real, co_off, with_bias) in enumerate(jobs):
         if isinstance(x, Checkpoint8) != held:
             raise ValueError("conv3x3_wgrad_multi: maps and checkpoints in one call")
-        if held:
-            x, sc = _req_checkpoint8(x, "x")
-            scales[j] = sc.data_ptr()
-            alive.append(sc)
-            if x.dim() != 4:
+        if id(x) not in checked:
+            if held and x.codes.dim() != 4:
                 raise ValueError("conv3x3_wgrad_multi: checkpoints of (N,H,W,C) maps")
-        else:
-            x = _req(x, torch.bfloat16, "x")
-        dz = _req(dz, torch.bfloat16, "dz")
-        alive += [x, dz]   # contiguous copies live until the launch is queued
+            checked[id(x)] = _req_checkpoint8(x, "x") if held else (_req(x, torch.bfloat16, "x"), None)
+        if id(dz) not in checked:
+            checked[id(dz)] = (_req(dz, torch.bfloat16, "dz"), None)
+        (x, sc), (dz, _) = checked[id(x)], checked[id(dz)]
+        if held:
+            scales[j] = sc.data_ptr()
         if shape is None:
             shape = tuple(x.shape[:3])
         if tuple(x.shape[:3]) != shape or tuple(dz.shape[:3]) != shape:
@@ -384,11 +384,23 @@ def _tile_channels(c: int) -> int:
     return 16 if c <= 16 else (32 if c <= 32 else 64)
 
 
+# conv_wgrad: a single map of up to this many pixels takes all slice pairs of a layer in one launch pair, in tiles of the largest pair.
+# What a padded tile computes in vain is little there, a launch pair more is not (160 -> 112 channels, kernel 1, split and merged:
+# 65 k pixels 51 and 35 us, 259 k 70 and 57, 522 k 111 and 127).
+WGRAD_MERGE_PIXELS = 1 << 18
+
+
 def conv_wgrad(srcs, dz: torch.Tensor, cin: int, cout: int, ksize: int):
     """Weight and bias gradient (dw (cout,cin,ksize,ksize), db (cout,), fp32) of a stride-1 layer with kernel 1 or 3 and any
     channel counts, whose input is the concatenation of ``srcs`` (NHWC bf16 maps or their checkpoints), from the gradient dz
     of its pre-activation output: one job per (<= 64 input, <= 64 output) channel slice pair, the channel windows read in
-    place.  SRHIP_NO_WGRAD_MULTI=1: a launch pair per job; SRHIP_NO_WGRAD_1X1=1: a 1x1 layer as the centre tap of a 3x3 one."""
+    place."""
+    return _conv_wgrad(srcs, dz, cin, cout, ksize, len(srcs) == 1 and dz.numel() // max(1, dz.shape[-1]) <= WGRAD_MERGE_PIXELS)
+
+
+def _conv_wgrad(srcs, dz: torch.Tensor, cin: int, cout: int, ksize: int, merge: bool = False):
+    """conv_wgrad with one tile shape for all slice pairs (``merge``) or a launch pair for each.  SRHIP_NO_WGRAD_MULTI=1: a launch
+    pair per job; SRHIP_NO_WGRAD_1X1=1: a 1x1 layer as the centre tap of a 3x3 one."""
     if ksize not in (1, 3):
         raise ValueError("conv_wgrad: kernel 1 or 3")
     if cin < 1 or cout < 1 or cout > dz.shape[-1] or cin > sum(t.shape[-1] for t in srcs):
@@ -402,6 +414,7 @@ def conv_wgrad(srcs, dz: torch.Tensor, cin: int, cout: int, ksize: int):
     # instead of one each per pair: on the 1/4 and 1/8 resolution maps a pair is a few microseconds of matrix work)
     groups = {}
     k0 = 0
+    top = _tile_channels(min(64, max(min(t.shape[-1], cin) for t in srcs))), _tile_channels(min(64, cout))
     for t in srcs:
         for a in range(0, t.shape[-1], 64):
             ci = min(a + 64, t.shape[-1]) - a
@@ -411,11 +424,11 @@ def conv_wgrad(srcs, dz: torch.Tensor, cin: int, cout: int, ksize: int):
             for o in range(0, cout, 64):
                 co = min(64, cout - o)
                 # the bias gradient rides on the first input slice's job (dz times ones on the MFMA pipe)
-                groups.setdefault((isinstance(t, Checkpoint8), _tile_channels(ci), _tile_channels(co)), []).append(
+                groups.setdefault((isinstance(t, Checkpoint8), top if merge else (_tile_channels(ci), _tile_channels(co))), []).append(
                     (t, a, ci_real, k0 + a, dz, o, co, o, k0 + a == 0))
         k0 += t.shape[-1]
     batch = 1 if os.environ.get("SRHIP_NO_WGRAD_MULTI", "0") == "1" else WGRAD_MAX_JOBS
-    for (_, ci_tile, co_tile), jobs in groups.items():
+    for (_, (ci_tile, co_tile)), jobs in groups.items():
         for b in range(0, len(jobs), batch):
             conv3x3_wgrad_multi(jobs[b:b + batch], dw, db, ci_tile, co_tile)
     return (dw if ksize == k_out else dw[:, :, 1:2, 1:2].contiguous()), db
@@ -1314,27 +1327,25 @@ def _norm_params(wb, c: int, name: str):
         return None, None
     if not isinstance(wb, (tuple, list)) or len(wb) != 2 or wb[0] is None:
         raise ValueError(f"{name}: expected (weight, bias or None)")
-    out = tuple(None if t is None else _req(t, torch.float32, f"{name} {k}") for t, k in zip(wb, ("weight", "bias")))
-    for t in out:
-        if t is not None and tuple(t.shape) != (c,):
-            raise ValueError(f"{name}: expected parameters of {c} channels, got {tuple(t.shape)}")
-    return out
+    w, b = _req(wb[0], torch.float32, name), None if wb[1] is None else _req(wb[1], torch.float32, name)
+    if w.dim() != 1 or w.shape[0] != c or (b is not None and b.shape != w.shape):
+        raise ValueError(f"{name}: expected parameters of {c} channels, got {[tuple(t.shape) for t in wb if t is not None]}")
+    return w, b
 
 
 def _norm_gate(gate: Optional[torch.Tensor], like: torch.Tensor):
     """(contiguous gate, mode, rows per gate, whether it is fp32 beside maps of another type)."""
     if gate is None:
         return None, _GATE_NONE, 0, 0
-    shape, c = tuple(like.shape), like.shape[-1]
-    rows = like.numel() // c
-    if tuple(gate.shape) == shape and gate.dtype in (like.dtype, torch.float32):
+    shape, c = like.shape, like.shape[-1]
+    if gate.shape == shape and gate.dtype in (like.dtype, torch.float32):
         return _req(gate, gate.dtype, "gate"), _GATE_MAP, 0, int(gate.dtype != like.dtype)
-    if tuple(gate.shape) == (c,):
-        per = rows
+    if gate.dim() == 1 and gate.shape[0] == c:
+        per = like.numel() // c
     elif like.dim() >= 3 and tuple(gate.shape) == (shape[0], c):
-        per = rows // max(1, shape[0])
+        per = like.numel() // c // max(1, shape[0])
     else:
-        raise ValueError(f"gate: expected shape {(c,)}, {(shape[0], c)} or {shape} (of the maps' type or fp32), got {tuple(gate.shape)} {gate.dtype}")
+        raise ValueError(f"gate: expected shape {(c,)}, {(shape[0], c)} or {tuple(shape)} (of the maps' type or fp32), got {tuple(gate.shape)} {gate.dtype}")
     gate = _req(gate, torch.float32, "gate")
     if per == 1:   # one row to a gate: a map
         return gate, _GATE_MAP, 0, int(like.dtype != torch.float32)
@@ -1433,10 +1444,13 @@ def norm_residual_bwd(h: Union[None, torch.Tensor, Checkpoint8], r: Union[None, 
     post_w, post_b = _norm_params(post, c, "post")
     pre_w, pre_b = _norm_params(pre, c, "pre")
     gate, mode, per, gate_f32 = _norm_gate(gate, like)
-    new = lambda t: None if t is None else torch.empty_like(t)  # noqa: E731
     like = dr if dr is not None else dn
-    g = NormResidualGrads(torch.empty_like(like), torch.empty_like(like) if h is not None else None, new(post_w), new(post_b), new(gate), new(scale_t),
-                          new(pre_w), new(pre_b))
+    # the parameters' gradients as the rows of one allocation
+    wanted = [post_w is not None, post_b is not None, pre_w is not None, pre_b is not None]
+    vectors = iter(torch.empty((sum(wanted), c), dtype=torch.float32, device=like.device).unbind(0)) if any(wanted) else iter(())
+    dpost_w, dpost_b, dpre_w, dpre_b = (next(vectors) if want else None for want in wanted)
+    g = NormResidualGrads(torch.empty_like(like), torch.empty_like(like) if h is not None else None, dpost_w, dpost_b,
+                          None if gate is None else torch.empty_like(gate), None if scale_t is None else torch.empty_like(scale_t), dpre_w, dpre_b)
     rows = like.numel() // c
     if rows == 0:
         for t in g:
