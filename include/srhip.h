@@ -610,6 +610,16 @@ SRHIP_API int srhip_relu_mask_checkpoint8(const void* dy, const void* codes, voi
 SRHIP_API int srhip_conv_wgrad_checkpoint8(const srhip_wgrad_job* jobs, const void* const* x_scales, int njobs, void* workspace, int n, int h,
                                            int w, int ci_pad, int co_pad, int w_i, int ksize, int accumulate, float scale, void* stream);
 
+/* Weight and bias gradient of a pointwise (1x1) layer of any width over npix pixels, as one GEMM:
+ *   dw[co][ci] = sum dz[pixel][co] * x[pixel][ci]  (fp32 (cout, cin)),  db[co] = sum dz[pixel][co]  (db may be NULL)
+ * x: bf16 pixels of x_cstride channels, or (x_scales not NULL) a checkpoint's codes; dz: bf16 pixels of dz_cstride channels.
+ * x_cstride is a multiple of 8 (16: codes), dz_cstride of 8; both maps start at multiples of 16 bytes; channels behind cin, cout
+ * are not used.  workspace: srhip_wgrad1x1_workspace_bytes(npix, cin, cout) bytes (none: NULL).  Written, not accumulated;
+ * deterministic.  From codes the result is that of the restored map, bit for bit. */
+SRHIP_API size_t srhip_wgrad1x1_workspace_bytes(long long npix, int cin, int cout);
+SRHIP_API int srhip_wgrad1x1(const void* x, const void* x_scales, const void* dz, float* dw, float* db, void* workspace, long long npix,
+                             int cin, int x_cstride, int cout, int dz_cstride, void* stream);
+
 /* ---------------------------------------------------------------------------
  * The norms around a residual block, fused with its gate and residual scale, over `rows` contiguous rows of c channels:
  *   p = N_post(h) (or h),   r = x + s * act(gate) * p,   n = N_pre(r)

@@ -125,6 +125,8 @@ _SIGNATURES = {
     "srhip_conv3x3_wgrad_multi": (c_int, [ctypes.POINTER(WgradJob), c_int, c_void_p] + [c_int] * 7 + [c_float, c_void_p]),
     "srhip_conv1x1_wgrad_multi": (c_int, [ctypes.POINTER(WgradJob), c_int, c_void_p] + [c_int] * 7 + [c_float, c_void_p]),
     "srhip_conv_wgrad_checkpoint8": (c_int, [ctypes.POINTER(WgradJob), ctypes.POINTER(c_void_p), c_int, c_void_p] + [c_int] * 8 + [c_float, c_void_p]),
+    "srhip_wgrad1x1_workspace_bytes": (c_size_t, [ctypes.c_longlong, c_int, c_int]),
+    "srhip_wgrad1x1": (c_int, [c_void_p] * 6 + [ctypes.c_longlong] + [c_int] * 4 + [c_void_p]),
     "srhip_checkpoint8_pack": (c_int, [c_void_p, c_int, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_void_p]),
     "srhip_checkpoint8_pack_signbits": (c_int, [c_void_p] * 4 + [c_int] * 3 + [c_void_p]),
     "srhip_checkpoint8_restore": (c_int, [c_void_p, c_void_p, c_void_p, c_int, ctypes.c_longlong, c_int, c_void_p]),

@@ -384,18 +384,41 @@ def _tile_channels(c: int) -> int:
     return 16 if c <= 16 else (32 if c <= 32 else 64)
 
 
-# conv_wgrad: a single map of up to this many pixels takes all slice pairs of a layer in one launch pair, in tiles of the largest pair.
-# What a padded tile computes in vain is little there, a launch pair more is not (160 -> 112 channels, kernel 1, split and merged:
-# 65 k pixels 51 and 35 us, 259 k 70 and 57, 522 k 111 and 127).
+# conv_wgrad: a single map of up to this many pixels takes all slice pairs of a 3x3 layer in one launch pair, in tiles of the
+# largest pair.  What a padded tile computes in vain is little there, a launch pair more is not (160 -> 112 channels, split and
+# merged: 65 k pixels 67 and 48 us, 259 k 119 and 111, 522 k 194 and 218).
 WGRAD_MERGE_PIXELS = 1 << 18
 
 
 def conv_wgrad(srcs, dz: torch.Tensor, cin: int, cout: int, ksize: int):
     """Weight and bias gradient (dw (cout,cin,ksize,ksize), db (cout,), fp32) of a stride-1 layer with kernel 1 or 3 and any
     channel counts, whose input is the concatenation of ``srcs`` (NHWC bf16 maps or their checkpoints), from the gradient dz
-    of its pre-activation output: one job per (<= 64 input, <= 64 output) channel slice pair, the channel windows read in
-    place."""
+    of its pre-activation output.  A pointwise layer of one source is a GEMM over the pixels (srhip_wgrad1x1); otherwise one job
+    per (<= 64 input, <= 64 output) channel slice pair, the channel windows read in place."""
+    if ksize == 1 and len(srcs) == 1:
+        return _wgrad1x1(srcs[0], dz, cin, cout)
     return _conv_wgrad(srcs, dz, cin, cout, ksize, len(srcs) == 1 and dz.numel() // max(1, dz.shape[-1]) <= WGRAD_MERGE_PIXELS)
+
+
+def _wgrad1x1(x, dz: torch.Tensor, cin: int, cout: int):
+    """conv_wgrad of a pointwise layer: x a (..., C) bf16 map or its checkpoint, dz (..., C')."""
+    held = isinstance(x, Checkpoint8)
+    x, sc = _req_checkpoint8(x, "x") if held else (_req(x, torch.bfloat16, "x"), None)
+    dz = _req(dz, torch.bfloat16, "dz")
+    if x.shape[:-1] != dz.shape[:-1]:
+        raise ValueError("conv_wgrad: x and dz disagree on their pixels")
+    if not 1 <= cin <= x.shape[-1] or not 1 <= cout <= dz.shape[-1]:
+        raise ValueError(f"conv_wgrad: {cin} -> {cout} channels of a source with {x.shape[-1]} and a gradient with {dz.shape[-1]}")
+    npix = dz.numel() // dz.shape[-1]
+    if npix == 0:
+        raise ValueError("conv_wgrad: empty maps")
+    dw = torch.empty((cout, cin, 1, 1), dtype=torch.float32, device=dz.device)
+    db = torch.empty((cout,), dtype=torch.float32, device=dz.device)
+    nbytes = lib.srhip_wgrad1x1_workspace_bytes(npix, cin, cout)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dz.device) if nbytes else None
+    check(lib.srhip_wgrad1x1(x.data_ptr(), _ptr(sc), dz.data_ptr(), dw.data_ptr(), db.data_ptr(), _ptr(ws), npix, cin, x.shape[-1], cout, dz.shape[-1],
+                             _stream()))
+    return dw, db
 
 
 def _conv_wgrad(srcs, dz: torch.Tensor, cin: int, cout: int, ksize: int, merge: bool = False):

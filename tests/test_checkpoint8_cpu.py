@@ -99,6 +99,14 @@ def test_c_entries_refuse_before_any_launch():
     job[0].x_cstride, job[0].x = 16, P + 8
     _refused(lib.srhip_conv_wgrad_checkpoint8(job, sc, 1, P, 1, 1, 1, 16, 16, 16, 3, 0, 1.0, None), "multiples of 16")
 
+    _refused(lib.srhip_wgrad1x1(P, P, P, P, P, P, 0, 16, 16, 16, 16, None), "empty layer")
+    _refused(lib.srhip_wgrad1x1(P, P, None, P, P, P, 8, 16, 16, 16, 16, None), "null pointer")
+    _refused(lib.srhip_wgrad1x1(P, P, P, P, P, P, 8, 16, 24, 16, 16, None), "multiples of 16")
+    _refused(lib.srhip_wgrad1x1(P, None, P, P, P, P, 8, 16, 16, 17, 16, None), "channels per pixel")
+    _refused(lib.srhip_wgrad1x1(P + 2, None, P, P, P, P, 8, 16, 16, 16, 16, None), "multiples of 16 bytes")
+    _refused(lib.srhip_wgrad1x1(P, None, P, P, P, None, 1 << 20, 16, 16, 16, 16, None), "null workspace")
+    assert lib.srhip_wgrad1x1_workspace_bytes(0, 16, 16) == 0 and lib.srhip_wgrad1x1_workspace_bytes(100, 16, 16) == 0
+
     a = dict(x=P, h=P, r=P, n=P, pre_weight=P, post_weight=P, rows=4, rows_per_gate=2, c=8, post=1, pre=1, eps=1e-6)
     for change, text in ((dict(c=0), "bad shape"), (dict(c=8193), "bad shape"), (dict(rows=-1), "bad shape"), (dict(dtype=2), "unknown type"),
                          (dict(kind=2), "unknown norm"), (dict(gate_mode=3), "unknown gate"), (dict(h=None, pre=0), "neither"),

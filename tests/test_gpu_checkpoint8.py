@@ -224,6 +224,40 @@ def test_weight_gradient_of_wide_layers(F, cin, cout, k):
     assert got[0].shape == (cout, cin, k, k) and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("cin,cout", [(1, 1), (16, 7), (33, 129), (128, 128), (130, 250), (320, 48), (257, 257)])
+@pytest.mark.parametrize("size", [(1, 1, 1), (1, 1, 31), (1, 3, 43), (2, 16, 16), (1, 70, 333)])
+def test_pointwise_weight_gradients(F, size, cin, cout):
+    """Every width and length of the pixel GEMM, from checkpoints and from maps: equal to each other, near to 64 bits; channels
+    behind the layer's, filled with NaN here, reach nothing."""
+    x, dz = _layer(*size, (cin + 15) // 16 * 16, (cout + 7) // 8 * 8, cin + cout + size[2])
+    x[..., cin:], dz[..., cout:] = float("nan"), float("nan")
+    ck = F.checkpoint8_pack(x)
+    rx = F.checkpoint8_restore(ck)
+    dw, db = F.checkpoint8_wgrad(ck, dz, cin, cout, 1)
+    dw2, db2 = F.conv_wgrad((rx,), dz, cin, cout, 1)
+    assert dw.shape == (cout, cin, 1, 1) and torch.equal(dw, dw2) and torch.equal(db, db2)
+    a, b = dz[..., :cout].reshape(-1, cout).double().cpu(), rx[..., :cin].reshape(-1, cin).double().cpu()
+    # fp32 sums of exact products: a term passes fewer additions than there are pixels, each rounding by 2^-24 of the sizes so far
+    bound = a.shape[0] * 2.0 ** -24
+    assert bool(((dw[:, :, 0, 0].double().cpu() - a.t() @ b).abs() <= bound * (a.abs().t() @ b.abs())).all())
+    assert bool(((db.double().cpu() - a.sum(0)).abs() <= bound * a.abs().sum(0)).all())
+
+
+def test_pointwise_weight_gradient_refusals(F):
+    x = torch.zeros(1, 4, 4, 24, dtype=torch.bfloat16, device="cuda")
+    ck = F.checkpoint8_pack(x)
+    with pytest.raises(RuntimeError, match="multiples of 16"):
+        F.checkpoint8_wgrad(ck, x, 24, 24, 1)
+    with pytest.raises(ValueError):
+        F.conv_wgrad((x,), x[:, :2], 24, 24, 1)
+    with pytest.raises(ValueError):
+        F.conv_wgrad((x,), x, 25, 24, 1)
+    with pytest.raises(ValueError):
+        F.conv_wgrad((x[:0],), x[:0], 24, 24, 1)
+    with pytest.raises(RuntimeError):
+        F.conv_wgrad((x,), torch.zeros(1, 4, 4, 10, dtype=torch.bfloat16, device="cuda"), 24, 10, 1)
+
+
 def test_weight_gradient_of_maps_and_checkpoints_side_by_side(F):
     xa, dz = _layer(1, 20, 70, 32, 64, 1)
     xb, _ = _layer(1, 20, 70, 64, 64, 2)
