@@ -373,6 +373,8 @@ class _ConvReluChain(Function):
     @staticmethod
     def forward(ctx, nsrc: int, cfgs, last_relu: bool, checkpoint: bool, *tensors: Tensor):
         srcs, wb = tensors[:nsrc], tensors[nsrc:]
+        if checkpoint and any(t.shape[-1] % 16 for t in srcs):
+            raise ValueError("autograd_ops.conv_relu_chain: checkpoints are kept of maps whose channel count is a multiple of 16")
         ws = [w.detach().float().contiguous() for w in wb[0::2]]
         ys, x = [], (tuple(srcs) if nsrc > 1 else srcs[0])
         for i, (w, b, (stride, padding)) in enumerate(zip(ws, wb[1::2], cfgs)):

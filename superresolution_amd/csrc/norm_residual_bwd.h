@@ -33,6 +33,7 @@ struct NormBwdParams {
     long long items;
     int segs;                                   // items per gate
     int c, groups, layer, post, pre, gate_mode, gate_f32, sigmoid, need_h, item_flush;
+    int direct;                                 // one item: its work-group writes the results, there is no second launch
     float scale, eps, inv_c;
 };
 
@@ -282,13 +283,19 @@ __global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG>())) void norm_r
             float part = 0.0f;
             sum_row_groups<C>(tile, l, a1, p.c, [&](const int ch, const float v) {
                 float slope;
+                const float gv = gate_value(p, s, ch, slope);
                 out[ch] = v;
-                if (p.dscale) part += v * gate_value(p, s, ch, slope) * (p.post_w ? p.post_w[ch] : 1.0f);
+                if (p.dscale) part += v * gv * (p.post_w ? p.post_w[ch] : 1.0f);
+                if (p.direct && p.dpost_w) p.dpost_w[ch] = scale * (gv * v);
             });
             sum_row_groups<C>(tile, l, a0, p.c, [&](const int ch, const float v) {
                 float slope;
+                const float gv = gate_value(p, s, ch, slope);
                 out[p.c + ch] = v;
-                if (p.dscale && p.post_b) part += v * gate_value(p, s, ch, slope) * p.post_b[ch];
+                if (p.dscale && p.post_b) part += v * gv * p.post_b[ch];
+                if (p.direct && p.dpost_b) p.dpost_b[ch] = scale * (gv * v);
+                if (p.direct && p.gate_mode == SRHIP_GATE_ROWS)   // out[ch] is this thread's own
+                    ((float*)p.dgate)[ch] = scale * slope * ((p.post_w ? p.post_w[ch] : 1.0f) * out[ch] + (p.post_b ? p.post_b[ch] : 0.0f) * v);
             });
             if (p.dscale) {
                 part = lanes_sum<64>(part);
@@ -297,15 +304,18 @@ __global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG>())) void norm_r
                 __syncthreads();
                 if (threadIdx.x == 0) {
                     for (int k = 1; k < C::THREADS / 64; ++k) part += tile[k];
-                    p.item_scale[item] = part;
+                    *(p.direct ? p.dscale : p.item_scale + item) = part;
                 }
             }
         }
     }
     if (p.pre) {
         float* out = p.wg_sums + (long long)blockIdx.x * 2 * p.c;
-        sum_row_groups<C>(tile, l, a_w, p.c, [&](const int ch, const float v) { out[ch] = v; });
-        sum_row_groups<C>(tile, l, a_b, p.c, [&](const int ch, const float v) { out[p.c + ch] = v; });
+        sum_row_groups<C>(tile, l, a_w, p.c, [&](const int ch, const float v) { (p.direct ? p.dpre_w : out)[ch] = v; });
+        sum_row_groups<C>(tile, l, a_b, p.c, [&](const int ch, const float v) {
+            if (!p.direct) out[p.c + ch] = v;
+            else if (p.dpre_b) p.dpre_b[ch] = v;
+        });
     }
 }
 

@@ -109,6 +109,7 @@ Plan plan_of(const srhip_norm_residual_bwd_args* a)
     // work-group at least, once every CU has one.
     long long grid = passes / 8;
     if (grid < cus) grid = passes < cus ? passes : cus;
+    if (passes <= 4) grid = 1;   // a few rows: one work-group and no second launch (four fp32 rows of 1024: 20.5 us a call, with two 24)
     if (grid > resident) grid = resident;
     const long long gates = a->gate_mode == SRHIP_GATE_ROWS ? a->rows / a->rows_per_gate : 1;
     const long long per_gate = a->rows / gates;
@@ -177,6 +178,7 @@ SRHIP_API int srhip_norm_residual_bwd(const srhip_norm_residual_bwd_args* a, voi
     p.c = a->c; p.groups = srhip_div_up(a->c, kCk8Group); p.layer = a->kind == SRHIP_NORM_LAYER; p.post = a->post; p.pre = a->pre;
     p.gate_mode = a->gate_mode; p.gate_f32 = a->dtype != SRHIP_DT_F32 && a->gate_f32; p.sigmoid = a->gate_sigmoid;
     p.need_h = need_h; p.item_flush = a->dh && (a->post || a->gate_mode == SRHIP_GATE_ROWS || a->dscale);
+    p.direct = q.items == 1;
     p.scale = a->scale; p.eps = a->eps; p.inv_c = 1.0f / (float)a->c;
     const long long gates = a->rows / p.rows_per_gate;
     const hipStream_t s = (hipStream_t)stream;
@@ -184,7 +186,7 @@ SRHIP_API int srhip_norm_residual_bwd(const srhip_norm_residual_bwd_args* a, voi
     const long long blocks = (5 + (p.gate_mode == SRHIP_GATE_ROWS ? gates : 0)) * cblocks;
     SRHIP_REQUIRE(blocks < (1ll << 31), "norm_residual_bwd: too many gates");
     const int launched = rows(a, &p, q, s);
-    if (launched != SRHIP_OK || (!p.pre && !p.item_flush)) return launched;
+    if (launched != SRHIP_OK || p.direct || (!p.pre && !p.item_flush)) return launched;
     hipLaunchKernelGGL(norm_residual_bwd_sums_kernel, dim3((unsigned)blocks), dim3(kCols * kParts), 0, s, p, q.grid, cblocks);
     return srhip_check_launch("norm_residual_bwd_sums_kernel");
 }

@@ -1393,6 +1393,16 @@ def _norm_options(kind: str, gate_act: str, eps: float, c: int, name: str) -> No
         raise ValueError(f"{name}: eps must not be negative")
 
 
+def _norm_saved(t, like: torch.Tensor, name: str):
+    """(data or codes, scales or None) of a map that was kept, or of its checkpoint."""
+    if t is None:
+        return None, None
+    data, sc = _req_checkpoint8(t, name) if isinstance(t, Checkpoint8) else (_req(t, like.dtype, name), None)
+    if data.shape != like.shape or (sc is not None and t.dtype != like.dtype):
+        raise ValueError(f"norm_residual_bwd: {name} is not of the gradients' shape and type")
+    return data, sc
+
+
 def norm_residual(x: torch.Tensor, h: Optional[torch.Tensor] = None, *, post=None, gate: Optional[torch.Tensor] = None, scale=1.0,
                   pre=None, kind: str = "layer", gate_act: str = "none", eps: float = 1e-6):
     """(r, n) with r = x + scale * gate_act(gate) * N_post(h) and n = N_pre(r), in one pass over (..., C) bf16 or fp32 maps: the
@@ -1454,16 +1464,8 @@ def norm_residual_bwd(h: Union[None, torch.Tensor, Checkpoint8], r: Union[None, 
     if h is None and (post is not None or gate is not None or scale_t is not None):
         raise ValueError("norm_residual_bwd: without a branch there is only the norm `pre`")
 
-    def saved(t, name):
-        if t is None:
-            return None, None
-        data, sc = _req_checkpoint8(t, name) if isinstance(t, Checkpoint8) else (_req(t, like.dtype, name), None)
-        if data.shape != like.shape or (sc is not None and t.dtype != like.dtype):
-            raise ValueError(f"norm_residual_bwd: {name} is not of the gradients' shape and type")
-        return data, sc
-
-    h_data, h_scales = saved(h, "h")
-    r_data, r_scales = saved(r if pre is not None else None, "r")
+    h_data, h_scales = _norm_saved(h, like, "h")
+    r_data, r_scales = _norm_saved(r if pre is not None else None, like, "r")
     post_w, post_b = _norm_params(post, c, "post")
     pre_w, pre_b = _norm_params(pre, c, "pre")
     gate, mode, per, gate_f32 = _norm_gate(gate, like)

@@ -66,6 +66,10 @@ class _MainNetwork(nn.Module):
 
 class SuperSampler(nn.Module):
     FR_CH, BF_CH, SR_CH = 32, 64, 64
+    # Training: set True on a model to keep the maps of its backward pass as 8-bit checkpoints (functional.checkpoint8_pack), about
+    # half the memory.  Output, data and bias gradients do not change (the ReLU patterns are kept exactly); weight gradients are
+    # formed from maps of 3 mantissa bits.
+    checkpoint_activations = False
 
     def __init__(self, frame_channels: int = 3, buffer_channels: int = 10, n_history: int = 1) -> None:
         super().__init__()
@@ -81,9 +85,6 @@ class SuperSampler(nn.Module):
         self.buffer_channels = buffer_channels
         self._init_parameters()
         self._packs: Dict[str, tuple] = {}
-        # training: keep the saved maps as 8-bit checkpoints (functional.checkpoint8_pack), about half the memory.  Output and data
-        # gradients do not change (the ReLU patterns are kept exactly); weight gradients are formed from maps of 3 mantissa bits
-        self.checkpoint_activations = False
         self.use_pair_kernel = os.environ.get("SRHIP_NO_PAIR", "0") != "1"
 
     def _init_parameters(self) -> None:

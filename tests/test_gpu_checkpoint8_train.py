@@ -89,6 +89,30 @@ def test_recurrent_network_trains_with_checkpoints():
     assert all(torch.equal(grads[0][1][k], grads[1][1][k]) for k in grads[0][1] if k.endswith("bias"))
 
 
+def test_attached_reducer_gets_the_checkpoint_gradients():
+    """Gradients accumulated straight into the flat buffer of the data-parallel reducer: those of the autograd path, added to
+    what is there."""
+    from superresolution_amd.dp import FlatGradAllReducer
+    m, batch = _model(), _batch(1, 8, 12)
+    m.checkpoint_activations = True
+    _, want = _step(m, *batch)
+    red = FlatGradAllReducer(m.parameters(), buckets=2).attach(m)
+    red.zero_grad()
+    out = m({"lr_frames": batch[0], "hr_buffers": batch[1]})["sr_frames"]
+    (out - batch[2]).abs().mean().backward()
+    red.all_reduce()
+    for k, p in m.named_parameters():
+        assert torch.equal(p.grad, want[k]), k
+
+
+def test_chains_refuse_widths_that_checkpoints_do_not_keep():
+    from superresolution_amd import autograd_ops as A
+    x = torch.zeros(1, 4, 4, 24, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    w, b = torch.zeros(16, 24, 1, 1, device="cuda", requires_grad=True), torch.zeros(16, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        A.conv_relu_chain(x, [(w, b, 1, 0)], checkpoint=True)
+
+
 # ---- a residual block
 def _block(x, p, c, checkpoint, gate):
     from superresolution_amd import autograd_ops as A

@@ -246,6 +246,58 @@ def test_results_repeat_and_streams_do_not_disturb_each_other(F):
             assert all(torch.equal(a, b) for a, b in zip(o, want))
 
 
+def test_first_call_of_a_width_inside_a_capture(F):
+    """What a kernel asks of the runtime on its first call is answered while a stream is being captured, too."""
+    x, h = (torch.randn(9, 5, 372, generator=torch.Generator().manual_seed(s)).cuda() for s in (1, 2))
+    w = torch.rand(372, generator=torch.Generator().manual_seed(3)).cuda()
+    how = dict(post=(w, None), pre=(w, w), kind="rms")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r, n = F.norm_residual(x, h, **how)
+        g = F.norm_residual_bwd(h, r, x, h, **how)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        want = F.norm_residual(x, h, **how)
+        wg = F.norm_residual_bwd(h, want[0], x, h, **how)
+        assert torch.equal(r, want[0]) and torch.equal(n, want[1])
+        assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(g, wg))
+
+
+def test_offsets_beyond_32_bits(F):
+    """2^31 elements and more: the last rows of a map equal the same rows on their own, forward, backward, packed, restored."""
+    rows, c, tail = (1 << 25) + 12345, 64, 4097
+    x = torch.empty((rows, c), dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(5))
+    assert x.numel() > 1 << 31
+    w, b = torch.rand(c, device="cuda") + 0.5, torch.rand(c, device="cuda")
+    how = dict(post=(w, b), gate=b, gate_act="sigmoid", scale=0.3, pre=(w, None))
+    t = x[-tail:]
+    r, n = F.norm_residual(x, x, **how)
+    rt, nt = F.norm_residual(t, t, **how)
+    assert torch.equal(r[-tail:], rt) and torch.equal(n[-tail:], nt)
+    del n
+    ck = F.checkpoint8_pack(x)
+    ct = F.checkpoint8_pack(t)
+    assert torch.equal(ck.codes[-tail:].view(torch.uint8), ct.codes.view(torch.uint8)) and torch.equal(ck.scales[-tail:], ct.scales)
+    y = F.checkpoint8_restore(ck)
+    assert torch.equal(y[-tail:], F.checkpoint8_restore(ct))
+    del y
+    m = F.relu_mask(x, ck)
+    assert torch.equal(m[-tail:], F.relu_mask(t, ct))
+    del m
+    g = F.norm_residual_bwd(ck, r, x, x, **how)
+    gt = F.norm_residual_bwd(ct, rt, t, t, **how)
+    assert torch.equal(g.dx[-tail:], gt.dx) and torch.equal(g.dh[-tail:], gt.dh)
+    del g, r
+    # a pointwise gradient that only the last pixels contribute to
+    dz = torch.zeros((rows, 16), dtype=torch.bfloat16, device="cuda")
+    dz[-tail:] = t[:, :16]
+    dw, _ = F.conv_wgrad((ck,), dz, c, 16, 1)
+    want = dz[-tail:].double().t() @ F.checkpoint8_restore(ct).double()
+    size = dz[-tail:].double().abs().t() @ F.checkpoint8_restore(ct).double().abs()
+    assert bool(((dw[:, :, 0, 0].double() - want).abs() <= tail * 2.0 ** -24 * size).all())
+
+
 def test_captured_and_replayed(F):
     def work(x, h, dr, dn, gate, scale, w, b):
         how = dict(post=(w, b), gate=gate, scale=scale, pre=(w, b), gate_act="sigmoid")
