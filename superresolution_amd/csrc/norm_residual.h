@@ -95,7 +95,7 @@ __device__ __forceinline__ float lane_sum(const Lane<C>& l, F&& term)
         float a = 0.0f;
 #pragma unroll
         for (int j = v * C::VEC; j < (v + 1) * C::VEC; ++j) {
-            if constexpr (C::ODD) a += l.counts[j] * term(j);   // (a row that holds a NaN has no sums but NaN)
+            if constexpr (C::ODD) a += l.mine(j) ? term(j) : 0.0f;   // (a choice, not a product: the term may be infinite)
             else a += term(j);
         }
         if (l.whole) s += a;

@@ -165,6 +165,18 @@ def test_rows_that_are_constant_zero_or_not_finite(F):
         assert torch.equal(a[fine], e[fine])
 
 
+@pytest.mark.parametrize("c", [64, 37, 5, 131])
+def test_an_infinity_leaves_the_rest_of_an_rms_row_at_zero(F, c):
+    """x / inf = 0 and inf / inf = NaN, at every place of the row and of its last vector."""
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.ones(c, c, dtype=dtype)
+        x.fill_diagonal_(float("inf"))
+        w = torch.ones(c).cuda()
+        _, n = F.norm_residual(x.cuda(), pre=(w, None), kind="rms")
+        eye = torch.eye(c, dtype=torch.bool)
+        assert bool(torch.isnan(n.cpu()[eye]).all()) and bool((n.cpu()[~eye] == 0).all())
+
+
 def test_a_large_mean_costs_no_digits(F):
     """Rows of 1000 +- 1: the spread is what counts."""
     d = _inputs((2, 9, 256), torch.float32, "layer", None, True, True, True, 5)
