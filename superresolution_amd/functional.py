@@ -271,6 +271,9 @@ _wgrad_ws = {}
 def _wgrad_workspace(device) -> torch.Tensor:
     """Partial-tile workspace of the weight-gradient kernel, one per (device, stream): launches on one stream are ordered
     and may share it; two streams running weight gradients at the same time must not (one partial tile set of 160 KB per CU: 42 MB each)."""
+    if torch.cuda.is_current_stream_capturing():
+        # a captured graph keeps a workspace of its own: graphs recorded on one stream may be replayed on several at once
+        return torch.empty((lib.srhip_conv3x3_wgrad_workspace_bytes(),), dtype=torch.uint8, device=device)
     key = (device, torch.cuda.current_stream(device).cuda_stream)
     ws = _wgrad_ws.get(key)
     if ws is None:

@@ -290,6 +290,32 @@ def test_on_another_stream_and_two_calls_at_once(F):
             assert torch.equal(o[0], ref[0]) and torch.equal(o[1], ref[1])
 
 
+def test_captured_weight_gradients_do_not_share_a_workspace(F):
+    """Two graphs recorded on one stream, replayed on two at once: from maps and from checkpoints, 3x3 and 1x1."""
+    data = [_layer(2, 90, 400, 64, 64, s) for s in (3, 4)]
+    cks = [F.checkpoint8_pack(x) for x, _ in data]
+
+    def work(i):
+        x, dz = data[i]
+        return F.conv_wgrad((x,), dz, 64, 64, 3) + F.conv_wgrad((x,), dz, 64, 64, 1) + F.checkpoint8_wgrad(cks[i], dz, 64, 64, 3) + F.checkpoint8_wgrad(cks[i], dz, 64, 64, 1)
+
+    want = [work(i) for i in range(2)]
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[0]):
+            outs.append(work(i))
+        graphs.append(g)
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
+
+
 def test_captured_and_replayed(F):
     """Two graphs of the whole run, replayed in turn with eager calls between: every replay equals the eager result."""
     def work(x, dz):
