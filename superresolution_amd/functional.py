@@ -1418,7 +1418,7 @@ def norm_residual(x: torch.Tensor, h: Optional[torch.Tensor] = None, *, post=Non
     gate_act:  "none" or "sigmoid".   scale: a number, or an fp32 tensor of one element.
     h None:    only the norm, r is x itself."""
     dt = _dtype_code(x.dtype, "x")
-    x = _req(x, x.dtype, "x")
+    given, x = x, _req(x, x.dtype, "x")
     if x.dim() < 2:
         raise ValueError("norm_residual: expected a (..., C) map")
     c = x.shape[-1]
@@ -1441,7 +1441,7 @@ def norm_residual(x: torch.Tensor, h: Optional[torch.Tensor] = None, *, post=Non
                          kind=_NORM_KINDS[kind], post=int(post is not None), pre=int(pre is not None), gate_mode=mode, gate_f32=gate_f32,
                          gate_sigmoid=_GATE_ACTS[gate_act], scale=scale_v, eps=eps)
     check(lib.srhip_norm_residual_fwd(a, _stream()))
-    return r, n
+    return given if h is None else r, n
 
 
 def norm_residual_bwd(h: Union[None, torch.Tensor, Checkpoint8], r: Union[None, torch.Tensor, Checkpoint8], dr: Optional[torch.Tensor],

@@ -177,6 +177,13 @@ def test_an_infinity_leaves_the_rest_of_an_rms_row_at_zero(F, c):
         assert bool(torch.isnan(n.cpu()[eye]).all()) and bool((n.cpu()[~eye] == 0).all())
 
 
+def test_without_a_branch_the_sum_is_the_map_that_was_given(F):
+    x = torch.randn(64, 33, device="cuda").t()                          # not contiguous: the norm reads a copy
+    w = torch.rand(64, device="cuda")
+    r, n = F.norm_residual(x, pre=(w, None))
+    assert r is x and torch.equal(n, F.norm_residual(x.contiguous(), pre=(w, None))[1])
+
+
 def test_a_large_mean_costs_no_digits(F):
     """Rows of 1000 +- 1: the spread is what counts."""
     d = _inputs((2, 9, 256), torch.float32, "layer", None, True, True, True, 5)
