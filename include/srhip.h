@@ -590,9 +590,9 @@ SRHIP_API int srhip_layernorm_cf_bwd_f32_static(const float* x, const float* wei
  * 8-bit activation checkpoints: what a training step keeps of a map for its backward pass (the maps that autograd saves for
  * loss.backward(), core/trainer.py:160).  A row of c channels (a pixel of an NHWC map, or any row of a matrix) is held as c
  * e4m3 codes and ceil(c / 32) bytes, one per 32 channels: s stands for the scale 2^(s - 127), 10 <= s <= 246, the smallest
- * power of two that brings the group's largest finite magnitude to 448 or less (one above 1.75 * 2^127 is kept as that).  code = x / scale, rounded to nearest even;
- * a value that is not 0 keeps a code that is not 0 (so [code > 0] is the ReLU pattern of a finite x); infinities and NaN
- * become NaN.  A decoded value is exact in bf16 and fp32.
+ * power of two that brings the group's largest finite magnitude to 448 or less (one above 1.75 * 2^127 is kept as that).
+ * code = x / scale, rounded to nearest even; a value that is not 0 keeps a code that is not 0 (so [code > 0] is the ReLU
+ * pattern of a finite x); infinities and NaN become NaN.  A decoded value is exact in bf16 and fp32.
  * Rows are contiguous; any c >= 1 and any alignment of the element type; rows == 0 does nothing.
  * ------------------------------------------------------------------------- */
 SRHIP_API int srhip_checkpoint8_pack(const void* x, int dtype /* SRHIP_DT_* */, void* codes, void* scales, long long rows, int c, void* stream);
