@@ -12,7 +12,7 @@ own = False
 DEV = "cuda"
 TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
 GROUP = 32        # channels that share a scale
-BIAS, LOWEST, HIGHEST = 127, 10, 246   # exponent byte of scale 1; the lowest and highest exponent bytes that a checkpoint holds
+BIAS, LOWEST = 127, 10   # exponent byte of scale 1; the lowest exponent byte that a checkpoint holds
 
 
 def listed():
@@ -78,7 +78,7 @@ def draw(rng):
 def _exponents(amax):
     """The exponent byte of a group whose largest magnitude is amax (fp32): the smallest scale that brings it to 448 or less."""
     b = amax.view(torch.int32)
-    return ((b >> 23) - 8 + ((b & 0x7FFFFF) > 0x600000).int()).clamp(LOWEST, HIGHEST)
+    return ((b >> 23) - 8 + ((b & 0x7FFFFF) > 0x600000).int()).clamp(min=LOWEST)
 
 
 def _spread(s, c):
@@ -94,7 +94,7 @@ def _encode(x):
     f = torch.where(f.isfinite(), f, torch.nan)
     amax = torch.nn.functional.pad(f.abs().nan_to_num(0.0), (0, g * GROUP - c)).unflatten(-1, (g, GROUP)).amax(-1)
     e = _exponents(amax)
-    codes = (f * _spread(_power(2 * BIAS - e), c)).clamp(-448, 448).to(torch.float8_e4m3fn)
+    codes = (f * _spread(_power(2 * BIAS - e), c)).to(torch.float8_e4m3fn)
     lost = (codes.view(torch.uint8) & 0x7F == 0) & (f != 0)
     codes = torch.where(lost, codes.view(torch.uint8) | 1, codes.view(torch.uint8)).view(torch.float8_e4m3fn)
     return codes, e.to(torch.uint8)
@@ -291,7 +291,7 @@ def exact(case, seed):
         tops = torch.stack([p.abs().amax(-1) for p in parts], -1)
         mantissa, power = torch.frexp(tops)                    # mantissa in [1/2, 1)
         e = torch.where(mantissa > 0.875, power - 8, power - 9)
-        e = torch.where(tops > 0, e, LOWEST - BIAS).clamp(LOWEST - BIAS, HIGHEST - BIAS)
+        e = torch.where(tops > 0, e, LOWEST - BIAS).clamp(min=LOWEST - BIAS)
         codes = torch.cat([torch.ldexp(p, -e[..., i:i + 1].to(D)) for i, p in enumerate(parts)], -1)
         if not case["bits"]:
             return codes, (e + BIAS).to(torch.uint8)
