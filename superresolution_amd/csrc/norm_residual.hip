@@ -28,7 +28,9 @@ struct NormParams {
     float scale, eps, inv_c;
 };
 
-// MAPG: the gate is a map.  Otherwise it is constant over runs of rows and sits, times the scale, in the post norm's parameters.
+// MAPG: the gate is a map.  Otherwise it is constant over runs of rows and held, times the scale, in registers.  It multiplies the
+// norm's result, weight and bias together, not the two on their own: an infinite gate is then an infinite term, as in the formula,
+// and not infinity times a bias of 0 or the difference of two infinities.
 template <class C, bool MAPG>
 __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormParams p)
 {
@@ -36,17 +38,15 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormPar
     __shared__ float scratch[row_sum_scratch<C>()];
     RowSum<C> sum{scratch, 0};
     const Lane<C> l(p.c);
-    float wpost[E], bpost[E], wpre[E], bpre[E];
+    float wpost[E], bpost[E], wpre[E], bpre[E], g[E];   // g: scale times gate
     load_params<C>(p.pre_w, l, 1.0f, wpre);
     load_params<C>(p.pre_b, l, 0.0f, bpre);
+    load_params<C>(p.post_w, l, 1.0f, wpost);
+    load_params<C>(p.post_b, l, 0.0f, bpost);
     const float scale = p.scale_ptr ? *p.scale_ptr : p.scale;
     long long gate_end = 0;   // first row that the gate held in registers does not belong to
-    if (p.gate_mode != SRHIP_GATE_ROWS) {
-        load_params<C>(p.post_w, l, 1.0f, wpost);
-        load_params<C>(p.post_b, l, 0.0f, bpost);
 #pragma unroll
-        for (int j = 0; j < E; ++j) { wpost[j] *= scale; bpost[j] *= scale; }
-    }
+    for (int j = 0; j < E; ++j) g[j] = scale;
 
     const long long first = blockIdx.x * p.wg_rows, last = p.wg_step || p.wg_rows > p.rows - first ? p.rows : first + p.wg_rows;
     for (long long base = first; base < last; base += p.wg_step ? p.wg_step : C::RPB) {
@@ -55,7 +55,6 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormPar
         const unsigned back = live ? 0u : (unsigned)((l.rg - (int)(p.rows - base - 1)) * p.c);
         const long long at = base * p.c * SIZE;
         rows_u32x4 qx[C::V], qh[C::V], qg[C::V];
-        float g[E];
         load_row<C>(p.x + at, l, back, qx);
         if (p.h) load_row<C>(p.h + at, l, back, qh);
         if constexpr (MAPG) {
@@ -65,14 +64,8 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormPar
             const long long s = (base + l.rg) / p.rows_per_gate;
             gate_end = (s + 1) * p.rows_per_gate;
             load_params<C>((const float*)p.gate + s * p.c, l, 0.0f, g);
-            load_params<C>(p.post_w, l, 1.0f, wpost);
-            load_params<C>(p.post_b, l, 0.0f, bpost);
 #pragma unroll
-            for (int j = 0; j < E; ++j) {
-                const float f = scale * (p.sigmoid ? sigmoid_f32(g[j]) : g[j]);
-                wpost[j] *= f;
-                bpost[j] *= f;
-            }
+            for (int j = 0; j < E; ++j) g[j] = scale * (p.sigmoid ? sigmoid_f32(g[j]) : g[j]);
         }
 
         float r[E];
@@ -87,11 +80,10 @@ __global__ __launch_bounds__(C::THREADS) void norm_residual_kernel(const NormPar
 #pragma unroll
                     for (int j = 0; j < E; ++j) g[j] = sigmoid_f32(g[j]);
 #pragma unroll
-                for (int j = 0; j < E; ++j) r[j] += g[j] * (h[j] * wpost[j] + bpost[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < E; ++j) r[j] += h[j] * wpost[j] + bpost[j];
+                for (int j = 0; j < E; ++j) g[j] *= scale;
             }
+#pragma unroll
+            for (int j = 0; j < E; ++j) r[j] += g[j] * (h[j] * wpost[j] + bpost[j]);
             if (live) store_row<C>(p.r + at, l, r);
         }
         if (p.pre) {

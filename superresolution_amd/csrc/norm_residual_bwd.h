@@ -49,6 +49,13 @@ __device__ __forceinline__ float gate_value(const NormBwdParams& p, const long l
     return a;
 }
 
+// Gradient of a gate that is constant over rows, from their sums A1 and A0; f: scale times the derivative of its activation
+__device__ __forceinline__ float gate_gradient(const NormBwdParams& p, const int ch, const float f, const float a1, const float a0)
+{
+    const float w = p.post_w ? p.post_w[ch] * a1 : a1;
+    return f * (p.post_b ? w + p.post_b[ch] * a0 : w);   // (no bias: nothing is added, an infinite A0 does not matter)
+}
+
 // Adds `acc` over the work-group's row groups, channel by channel, and hands (channel, sum) to `put`; every thread calls it.
 template <class C, class F>
 __device__ __forceinline__ void sum_row_groups(float* tile, const Lane<C>& l, const float* acc, const int c, F&& put)
@@ -163,16 +170,14 @@ __global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG>())) void norm_r
     __shared__ float tile[row_groups_tile<C>()];
     RowSum<C> sum{scratch, 0};
     const Lane<C> l(p.c);
-    float wpre[E], sw[E];   // sw: scale (and, constant over an item, the gate) times the post norm's weight
-    float sb[MAPG ? E : 1];
+    float wpre[E], sw[E];   // sw: scale and gate, constant over an item, times the post norm's weight; of a gate map the weight alone
+    float sb[MAPG ? E : 1]; // a gate map: the post norm's bias
     float a_w[E], a_b[E], a1[E], a0[E];
     load_params<C>(p.pre_w, l, 1.0f, wpre);
     const float scale = p.scale_ptr ? *p.scale_ptr : p.scale;
     if constexpr (MAPG) {
         load_params<C>(p.post_w, l, 1.0f, sw);
         load_params<C>(p.post_b, l, 0.0f, sb);
-#pragma unroll
-        for (int j = 0; j < E; ++j) { sw[j] *= scale; sb[j] *= scale; }
     }
 #pragma unroll
     for (int j = 0; j < E; ++j) a_w[j] = a_b[j] = 0.0f;
@@ -248,7 +253,7 @@ __global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG>())) void norm_r
                 float dg[E];
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
-                    dg[j] = d[j] * (h[j] * sw[j] + sb[j]);
+                    dg[j] = scale * d[j] * (h[j] * sw[j] + sb[j]);   // (the scale outside: an infinite one meets no bias of 0)
                     if (p.sigmoid) dg[j] *= g[j] * (1.0f - g[j]);
                     d[j] *= g[j];
                 }
@@ -266,7 +271,7 @@ __global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG>())) void norm_r
 #pragma unroll
                 for (int j = 0; j < E; ++j) { a1[j] += d[j] * h[j]; a0[j] += d[j]; }
 #pragma unroll
-            for (int j = 0; j < E; ++j) d[j] *= sw[j];
+            for (int j = 0; j < E; ++j) d[j] = MAPG ? d[j] * scale * sw[j] : d[j] * sw[j];
             if (p.post) {
                 float m1 = 0.0f, m2 = lane_sum<C>(l, [&](int j) { return d[j] * h[j]; });
                 if (p.layer) m1 = lane_sum<C>(l, [&](int j) { return d[j]; });
@@ -295,7 +300,7 @@ __global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG>())) void norm_r
                 if (p.dscale && p.post_b) part += v * gv * p.post_b[ch];
                 if (p.direct && p.dpost_b) p.dpost_b[ch] = scale * (gv * v);
                 if (p.direct && p.gate_mode == SRHIP_GATE_ROWS)   // out[ch] is this thread's own
-                    ((float*)p.dgate)[ch] = scale * slope * ((p.post_w ? p.post_w[ch] : 1.0f) * out[ch] + (p.post_b ? p.post_b[ch] : 0.0f) * v);
+                    ((float*)p.dgate)[ch] = gate_gradient(p, ch, scale * slope, out[ch], v);
             });
             if (p.dscale) {
                 part = lanes_sum<64>(part);

@@ -85,8 +85,7 @@ __global__ __launch_bounds__(kCols * kParts) void norm_residual_bwd_sums_kernel(
     else {
         float slope;
         gate_value(p, section - 5, ch, slope);
-        ((float*)p.dgate)[(long long)(section - 5) * p.c + ch] =
-            scale * slope * ((p.post_w ? p.post_w[ch] : 1.0f) * a + (p.post_b ? p.post_b[ch] : 0.0f) * b);
+        ((float*)p.dgate)[(long long)(section - 5) * p.c + ch] = gate_gradient(p, ch, scale * slope, a, b);
     }
 }
 

@@ -348,3 +348,66 @@ def test_captured_and_replayed(F):
             torch.cuda.synchronize()
             for a, b in zip(outs[i], want):
                 assert (a is None and b is None) or torch.equal(a, b)
+
+
+def _same_with_infinities(got, want, size, k, what):
+    """Infinities and NaN where the definition has them, the rest near to it."""
+    got, w = got.cpu().double(), want.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(w)), what
+    inf = torch.isinf(w)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], w[inf]), what
+    fine = torch.isfinite(w)
+    u = torch.finfo(torch.bfloat16 if what[1] == torch.bfloat16 else torch.float32).eps / 2
+    tol = (1 + u) * k * 2.0 ** -24 * size[fine] + u * w[fine].abs() + 1e-38
+    assert bool(((got[fine] - w[fine]).abs() <= tol).all()), what
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gate", ["channel", "sample", "map", "map32"])
+@pytest.mark.parametrize("kind,post,bias", [("rms", True, False), ("rms", True, True), ("layer", True, True), ("rms", False, False)])
+def test_an_infinite_gate_is_an_infinite_term(F, kind, post, bias, gate, dtype):
+    """Infinities and NaN among the gates reach their own channels, with the branch's sign: no infinity meets a bias on its own.
+    Gradients: the gates' are finite (no gate is in them), the branch's are infinite where the gate is."""
+    d = _inputs((3, 7, 40), dtype, kind, gate, post, False, bias, 21)
+    for i, v in ((5, float("inf")), (6, -float("inf")), (7, float("nan"))):
+        d["gate"][..., i] = v
+    r, _ = F.norm_residual(_dev(d["x"]), _dev(d["h"]), post=_dev(d["post"]), gate=_dev(d["gate"]), scale=0.5, kind=kind)
+    (want, _), (size, _) = orc.norm_residual(d["x"], d["h"], d["post"], d["gate"], 0.5, None, kind, "none")
+    assert bool(torch.isinf(want[..., 5:7]).all())
+    _same_with_infinities(r, want, size, K, ("r", dtype))
+    g = F.norm_residual_bwd(_dev(d["h"]), None, _dev(d["dr"]), None, post=_dev(d["post"]), gate=_dev(d["gate"]), scale=0.5, kind=kind)
+    want, size = orc.norm_residual_bwd(d["h"], None, d["dr"], None, d["post"], d["gate"], 0.5, None, kind, "none", False)
+    assert bool(torch.isfinite(want["dgate"]).all())
+    dt = dtype if gate == "map" else torch.float32
+    _same_with_infinities(g.dgate, want["dgate"], size["dgate"], K_ROWS, ("dgate", dt))
+    if not post:
+        _same_with_infinities(g.dh, want["dh"], size["dh"], K, ("dh", dtype))
+
+
+@pytest.mark.parametrize("gate", [None, "channel", "sample", "map"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_an_infinite_scale_and_infinite_gradients(F, bias, gate):
+    """The residual scale at infinity: every term is infinite, with its sign; the gate's gradient too.  An infinite gradient of the sum
+    reaches the gate's gradient as an infinity where the norm has no bias."""
+    d = _inputs((2, 9, 24), torch.float32, "rms", gate, True, False, bias, 22)
+    for scale in (float("inf"), torch.tensor(float("inf"))):
+        how = dict(post=_dev(d["post"]), gate=_dev(d["gate"]), scale=_dev(scale) if isinstance(scale, torch.Tensor) else scale, kind="rms")
+        r, _ = F.norm_residual(_dev(d["x"]), _dev(d["h"]), **how)
+        (want, _), _ = orc.norm_residual(d["x"], d["h"], d["post"], d["gate"], scale, None, "rms", "none")
+        assert bool(torch.isinf(want).all()) and torch.equal(r.cpu().double(), want)
+        if gate == "map" or (gate and not bias):
+            g = F.norm_residual_bwd(_dev(d["h"]), None, _dev(d["dr"]), None, **how)
+            want = _p_of(d, "rms") * d["dr"].double()
+            want = torch.inf * (want if gate == "map" else want.sum((0, 1)) if gate == "channel" else want.sum(1))
+            assert torch.equal(g.dgate.cpu().double(), want)
+    if gate in ("channel", "sample") and not bias:
+        d["dr"][1, 4, 3] = float("inf")
+        g = F.norm_residual_bwd(_dev(d["h"]), None, _dev(d["dr"]), None, post=_dev(d["post"]), gate=_dev(d["gate"]), kind="rms")
+        got = (g.dgate if gate == "channel" else g.dgate[1]).cpu()
+        assert float(got[3]) == torch.inf * float(_p_of(d, "rms")[1, 4, 3]) and int(torch.isfinite(got).sum()) == 23
+
+
+def _p_of(d, kind):
+    """The branch behind its norm, in 64 bits."""
+    w, b = d["post"]
+    return orc._norm(d["h"].double(), (w.double(), None if b is None else b.double()), kind, 1e-6)[2]
