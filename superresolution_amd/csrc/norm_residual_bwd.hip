@@ -7,22 +7,26 @@ using namespace srhip_norm;
 namespace {
 
 // Adds the sums of work-groups and items: 32 columns to a block, 32 thread groups taking every 32nd sum, then theirs in
-// order.  Block b: section b / cblocks (0, 1: dw_pre, db_pre; 2, 3: dw_post, db_post; 4: ds; 5 + i: gate i) of 32 channels.
+// order.  Block b: section b / cblocks (0, 1: dw_pre, db_pre; 2, 3: dw_post, db_post; 4: ds; 5 + i: gate i) of 32 channels.  A
+// launch has fewer than 2^32 threads along x: gates beyond kMaxBlocks lie along y, `gate_row` to each of its rows.
 // A chain of dependent-looking loads is what bounds it: a thousand sums in 32 steps of eight loads each (4.6 MB; 64 columns and
 // 16 groups, with a division by the items of a gate in every step, took 34 us for 64 channels, this 5).
 constexpr int kCols = 32, kParts = 32;
-__global__ __launch_bounds__(kCols * kParts) void norm_residual_bwd_sums_kernel(const NormBwdParams p, const int nwg, const int cblocks)
+constexpr long long kMaxBlocks = (1ll << 32) / (kCols * kParts) - 1;
+__global__ __launch_bounds__(kCols * kParts) void norm_residual_bwd_sums_kernel(const NormBwdParams p, const int nwg, const int cblocks, const long long gates, const long long gate_row)
 {
     __shared__ float red[2][kParts][kCols];
     const int col = threadIdx.x % kCols, part = threadIdx.x / kCols;
     const int section = (int)(blockIdx.x / (unsigned)cblocks);
     const int ch = (int)(blockIdx.x % (unsigned)cblocks) * kCols + col;
     const bool in = ch < p.c;
+    const long long gate = section - 5 + blockIdx.y * gate_row;
+    if (section < 5 ? blockIdx.y != 0 : gate >= gates) return;   // uniform over the block, as all that follow
     const float scale = p.scale_ptr ? *p.scale_ptr : p.scale;
     float a = 0.0f, b = 0.0f;
     if (section < 2) {
         float* dst = section == 0 ? p.dpre_w : p.dpre_b;
-        if (dst == nullptr) return;   // uniform over the block, as all that follow
+        if (dst == nullptr) return;
         if (in) {
             const float* src = p.wg_sums + section * p.c + ch;
 #pragma unroll 8
@@ -58,9 +62,8 @@ __global__ __launch_bounds__(kCols * kParts) void norm_residual_bwd_sums_kernel(
 #pragma unroll 4
         for (long long k = threadIdx.x; k < p.items; k += kCols * kParts) a += p.item_scale[k];
     } else {
-        const long long s = section - 5;
         if (in) {
-            const float* src = p.item_sums + s * p.segs * 2 * p.c + ch;
+            const float* src = p.item_sums + gate * p.segs * 2 * p.c + ch;
 #pragma unroll 8
             for (int k = part; k < p.segs; k += kParts) {
                 a += src[2ll * k * p.c];
@@ -84,8 +87,8 @@ __global__ __launch_bounds__(kCols * kParts) void norm_residual_bwd_sums_kernel(
     else if (section < 4) (section == 2 ? p.dpost_w : p.dpost_b)[ch] = scale * a;
     else {
         float slope;
-        gate_value(p, section - 5, ch, slope);
-        ((float*)p.dgate)[(long long)(section - 5) * p.c + ch] = gate_gradient(p, ch, scale * slope, a, b);
+        gate_value(p, gate, ch, slope);
+        ((float*)p.dgate)[gate * p.c + ch] = gate_gradient(p, ch, scale * slope, a, b);
     }
 }
 
@@ -179,14 +182,16 @@ SRHIP_API int srhip_norm_residual_bwd(const srhip_norm_residual_bwd_args* a, voi
     p.need_h = need_h; p.item_flush = a->dh && (a->post || a->gate_mode == SRHIP_GATE_ROWS || a->dscale);
     p.direct = q.items == 1;
     p.scale = a->scale; p.eps = a->eps; p.inv_c = 1.0f / (float)a->c;
-    const long long gates = a->rows / p.rows_per_gate;
+    const long long gates = p.gate_mode == SRHIP_GATE_ROWS ? a->rows / p.rows_per_gate : 0;
     const hipStream_t s = (hipStream_t)stream;
     const int cblocks = srhip_div_up(p.c, kCols);
-    const long long blocks = (5 + (p.gate_mode == SRHIP_GATE_ROWS ? gates : 0)) * cblocks;
-    SRHIP_REQUIRE(blocks < (1ll << 31), "norm_residual_bwd: too many gates");
+    const long long most = kMaxBlocks / cblocks - 5, gate_row = gates < most ? gates : most;
+    const long long gate_rows = gates > gate_row ? (gates + gate_row - 1) / gate_row : 1;
+    SRHIP_REQUIRE(gate_rows < (1ll << 16), "norm_residual_bwd: too many gates");
     const int launched = rows(a, &p, q, s);
     if (launched != SRHIP_OK || p.direct || (!p.pre && !p.item_flush)) return launched;
-    hipLaunchKernelGGL(norm_residual_bwd_sums_kernel, dim3((unsigned)blocks), dim3(kCols * kParts), 0, s, p, q.grid, cblocks);
+    hipLaunchKernelGGL(norm_residual_bwd_sums_kernel, dim3((unsigned)((5 + gate_row) * cblocks), (unsigned)gate_rows), dim3(kCols * kParts), 0, s, p, q.grid,
+                       cblocks, gates, gate_row);
     return srhip_check_launch("norm_residual_bwd_sums_kernel");
 }
 

@@ -411,3 +411,30 @@ def _p_of(d, kind):
     """The branch behind its norm, in 64 bits."""
     w, b = d["post"]
     return orc._norm(d["h"].double(), (w.double(), None if b is None else b.double()), kind, 1e-6)[2]
+
+
+@pytest.mark.parametrize("c,gates", [(8192, 16397), (4096, 2 * 32763 + 5)])
+def test_gates_beyond_one_row_of_the_launch(F, c, gates):
+    """Gates times channel blocks beyond 2^22 (2^32 threads): the second and third row of the launch; the first and last gates' gradients equal
+    those of the same gates on their own (an item to a gate in both, added in the same order)."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    g = torch.Generator(device="cuda").manual_seed(9)
+    h, dr = (torch.empty((gates, 2, c), dtype=torch.bfloat16, device="cuda").normal_(generator=g) for _ in range(2))
+    gate, w = torch.empty((gates, c), device="cuda").normal_(generator=g), torch.rand(c, device="cuda", generator=g)
+    got = F.norm_residual_bwd(h, None, dr, None, post=(w, None), gate=gate, gate_act="sigmoid", kind="rms").dgate
+    per = (1 << 22) // (c // 32)
+    for lo in (0, per - 300, gates - 600):
+        part = slice(lo, lo + 600)
+        want = F.norm_residual_bwd(h[part], None, dr[part], None, post=(w, None), gate=gate[part], gate_act="sigmoid", kind="rms").dgate
+        assert torch.equal(got[part], want), lo
+    off = torch.zeros(gates, device="cuda")
+    for lo in range(0, gates, 4096):          # every gate against its sum, in 32 bits
+        part = slice(lo, lo + 4096)
+        hat = h[part].float()
+        p = dr[part].float() * (hat / (hat.square().mean(-1, keepdim=True) + 1e-6).sqrt()) * w
+        a = torch.sigmoid(gate[part])
+        # the sums' arithmetic, and 1 - a, whose error is that of a: two roundings of at most one unit in the last place
+        size = p.abs().sum(1) * (K * a * (1 - a) + 4 * a)
+        off[part] = ((got[part] - p.sum(1) * a * (1 - a)).abs() / (size * 2.0 ** -24 + 1e-30)).amax(-1)
+    assert float(off.max()) < 2               # once on each side
