@@ -195,8 +195,14 @@ __global__ __launch_bounds__(kThreads) void relu_mask_checkpoint8_kernel(const c
     store_row16<__bf16>(out + 2 * i, d, nv);
 }
 
-// rows of one launch: units (rows times groups) stay below 2^31
-long long slab_rows(const int groups) { return ((1ll << 31) - 1) / groups; }
+// A launch has fewer than 2^32 threads, and units (rows times groups) that fit 31 bits: the rows of one launch whose units take
+// `lanes` lanes each.
+constexpr long long kMaxBlocks = (1ll << 32) / kThreads - 1;
+long long slab_rows(const int groups, const int lanes)
+{
+    const long long units = kMaxBlocks * (kThreads / lanes);
+    return (units < (1ll << 31) ? units : (1ll << 31) - 1) / groups;
+}
 
 template <class T, int LANES>
 int pack_slab(const char* x, unsigned char* codes, unsigned char* scales, const long long units, const int c, const int groups, hipStream_t s)
@@ -212,34 +218,34 @@ int restore_slab(const unsigned char* codes, const unsigned char* scales, char* 
                        codes, scales, y, units, c, groups);
     return srhip_check_launch("checkpoint8_restore_kernel");
 }
+// Calls f(first row, units, lanes of a unit) for each launch over `rows` rows of c channels.
 // (Two 540 x 959 maps of ten fp32 channels: with four lanes to a row 17 us, with two 13.6.)
-template <class T>
-int pack_rows(const char* x, unsigned char* codes, unsigned char* scales, const long long rows, const int c, hipStream_t s)
+template <class F>
+int by_slabs(const long long rows, const int c, const int groups, F&& f)
 {
-    const int groups = srhip_div_up(c, kCk8Group);
-    for (long long r = 0; r < rows; r += slab_rows(groups)) {
-        const long long units = (rows - r < slab_rows(groups) ? rows - r : slab_rows(groups)) * groups;
-        const char* xs = x + r * c * RowVec<T>::SIZE;
-        unsigned char *cs = codes + r * c, *ss = scales + r * groups;
-        const int rc = c <= 8 ? pack_slab<T, 1>(xs, cs, ss, units, c, groups, s) : c <= 16 ? pack_slab<T, 2>(xs, cs, ss, units, c, groups, s)
-                                                                                           : pack_slab<T, 4>(xs, cs, ss, units, c, groups, s);
+    const int lanes = c <= 8 ? 1 : c <= 16 ? 2 : 4;
+    const long long most = slab_rows(groups, lanes);
+    for (long long r = 0; r < rows; r += most) {
+        const int rc = f(r, (rows - r < most ? rows - r : most) * groups, lanes);
         if (rc != SRHIP_OK) return rc;
     }
     return SRHIP_OK;
 }
 template <class T>
+int pack_rows(const char* x, unsigned char* codes, unsigned char* scales, const long long rows, const int c, hipStream_t s)
+{
+    const int groups = srhip_div_up(c, kCk8Group);
+    return by_slabs(rows, c, groups, [&](const long long r, const long long units, const int lanes) {
+        return (lanes == 1 ? pack_slab<T, 1> : lanes == 2 ? pack_slab<T, 2> : pack_slab<T, 4>)(x + r * c * RowVec<T>::SIZE, codes + r * c, scales + r * groups, units, c, groups, s);
+    });
+}
+template <class T>
 int restore_rows(const unsigned char* codes, const unsigned char* scales, char* y, const long long rows, const int c, hipStream_t s)
 {
     const int groups = srhip_div_up(c, kCk8Group);
-    for (long long r = 0; r < rows; r += slab_rows(groups)) {
-        const long long units = (rows - r < slab_rows(groups) ? rows - r : slab_rows(groups)) * groups;
-        const unsigned char *cs = codes + r * c, *ss = scales + r * groups;
-        char* ys = y + r * c * RowVec<T>::SIZE;
-        const int rc = c <= 8 ? restore_slab<T, 1>(cs, ss, ys, units, c, groups, s) : c <= 16 ? restore_slab<T, 2>(cs, ss, ys, units, c, groups, s)
-                                                                                              : restore_slab<T, 4>(cs, ss, ys, units, c, groups, s);
-        if (rc != SRHIP_OK) return rc;
-    }
-    return SRHIP_OK;
+    return by_slabs(rows, c, groups, [&](const long long r, const long long units, const int lanes) {
+        return (lanes == 1 ? restore_slab<T, 1> : lanes == 2 ? restore_slab<T, 2> : restore_slab<T, 4>)(codes + r * c, scales + r * groups, y + r * c * RowVec<T>::SIZE, units, c, groups, s);
+    });
 }
 
 }  // namespace
@@ -266,7 +272,7 @@ SRHIP_API int srhip_checkpoint8_pack_signbits(const void* x, void* codes, void* 
     const int wgroups = srhip_div_up(w, 32);
     const long long nwords = (long long)n * h * wgroups;
     const long long blocks = (nwords + kThreads / 64 - 1) / (kThreads / 64);
-    SRHIP_REQUIRE(blocks < (1ll << 31), "checkpoint8_pack_signbits: map too large");
+    SRHIP_REQUIRE(blocks <= kMaxBlocks, "checkpoint8_pack_signbits: map too large");   // (2^31 pixels of whole groups of 32: 256 GB)
     hipLaunchKernelGGL(checkpoint8_pack_signbits_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, (hipStream_t)stream, (const char*)x,
                        (unsigned char*)codes, (unsigned char*)scales, (unsigned*)signbits, nwords, w, wgroups);
     return srhip_check_launch("checkpoint8_pack_signbits_kernel");
@@ -286,11 +292,15 @@ SRHIP_API int srhip_relu_mask_checkpoint8(const void* dy, const void* codes, voi
 {
     if (n == 0) return SRHIP_OK;
     SRHIP_REQUIRE(dy && codes && out, "relu_mask_checkpoint8: null pointer");
-    const size_t blocks = (n + 8 * kThreads - 1) / (8 * kThreads);
-    SRHIP_REQUIRE(blocks < ((size_t)1 << 31), "relu_mask_checkpoint8: map too large");
-    hipLaunchKernelGGL(relu_mask_checkpoint8_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, (hipStream_t)stream, (const char*)dy,
-                       (const unsigned char*)codes, (char*)out, (long long)n);
-    return srhip_check_launch("relu_mask_checkpoint8_kernel");
+    constexpr size_t kMost = (size_t)kMaxBlocks * 8 * kThreads;   // elements of a launch
+    for (size_t i = 0; i < n; i += kMost) {
+        const size_t m = n - i < kMost ? n - i : kMost;
+        hipLaunchKernelGGL(relu_mask_checkpoint8_kernel, dim3((unsigned)((m + 8 * kThreads - 1) / (8 * kThreads))), dim3(kThreads), 0, (hipStream_t)stream,
+                           (const char*)dy + 2 * i, (const unsigned char*)codes + i, (char*)out + 2 * i, (long long)m);
+        const int rc = srhip_check_launch("relu_mask_checkpoint8_kernel");
+        if (rc != SRHIP_OK) return rc;
+    }
+    return SRHIP_OK;
 }
 
 }  // extern "C"

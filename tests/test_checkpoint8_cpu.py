@@ -148,3 +148,9 @@ def test_python_entries_refuse_host_tensors_and_wrong_types():
         F.norm_residual_bwd(x, x, x, x)
     with pytest.raises(ValueError):
         F.conv_wgrad((x[None],), x[None], 64, 64, 5)
+
+
+def test_launches_of_too_many_threads_are_refused_on_the_host():
+    from superresolution_amd._lib import lib
+    # one pixel to a group of 32: 2^26 groups, 2^32 threads
+    _refused(lib.srhip_checkpoint8_pack_signbits(P, P, P, P, 1024, 65536, 1, None), "too large")

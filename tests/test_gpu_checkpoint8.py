@@ -343,3 +343,50 @@ def test_captured_and_replayed(F):
             torch.cuda.synchronize()
             for a, b in zip(outs[i], want):
                 assert torch.equal(a, b)
+
+
+def _room(gib):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GB")
+
+
+@pytest.mark.parametrize("rows,c,dtype", [((1 << 30) // 2 + 77, 64, torch.bfloat16), ((1 << 31) + 4321, 1, torch.bfloat16), ((1 << 31) + 513, 9, torch.bfloat16)])
+def test_maps_that_take_more_than_one_launch(F, rows, c, dtype):
+    """More rows than a launch holds (2^32 threads, or 2^31 units): values at the start, around where the launches meet and at the end are
+    those of the same rows on their own, zeros in between; saved, brought back, as a ReLU mask."""
+    _room(190)
+    groups = (c + 31) // 32
+    lanes = 1 if c <= 8 else 2 if c <= 16 else 4
+    meet = min((1 << 32) // lanes, 1 << 31) // groups
+    places = [0, meet - 700, rows - 400]
+    blocks = [_values((min(1000, rows - p), c), dtype, p % 97).cuda() for p in places]
+    x = torch.zeros((rows, c), dtype=dtype, device="cuda")
+    for p, b in zip(places, blocks):
+        x[p:p + len(b)] = b
+    ck = F.checkpoint8_pack(x)
+    dy = torch.empty_like(x).fill_(3.0) if x.numel() < 1 << 35 else None
+    del x
+    want = [F.checkpoint8_pack(b) for b in blocks]
+
+    def same(t, of):
+        for p, w in zip(places, want):
+            b = of(w)
+            n = min([len(b)] + [q - p for q in places if q > p])       # where two overlap the later one stands
+            assert torch.equal(t[p:p + n], b[:n]), p
+        for lo in range(1000, places[1], 1 << 24):
+            assert not bool(t[lo:min(lo + (1 << 24), places[1])].any()), lo
+
+    same(ck.codes.view(torch.uint8), lambda w: w.codes.view(torch.uint8))
+    assert torch.equal(ck.scales[-400:], want[-1].scales[-400:])
+    y = F.checkpoint8_restore(ck)
+    same(y.view(torch.int16), lambda w: F.checkpoint8_restore(w).view(torch.int16))
+    if dy is None:
+        dy = y      # in place: the map itself where it is positive
+        mask = lambda w: F.relu_mask(F.checkpoint8_restore(w), w).view(torch.int16)  # noqa: E731
+    else:
+        del y
+        mask = lambda w: F.relu_mask(torch.full(w.codes.shape, 3.0, dtype=dtype, device="cuda"), w).view(torch.int16)  # noqa: E731
+    same(F.relu_mask(dy, ck, out=dy).view(torch.int16), mask)
+    del ck, dy
+    torch.cuda.empty_cache()
