@@ -103,10 +103,12 @@ int launch_rows(NormParams p, hipStream_t stream)
     if (C::TPR <= 64 && C::E <= 8) {
         // Short rows: eight passes to a work-group, enough to pay for its parameters, and as many work-groups as that makes
         // (64 channels of four 1024^2 crops: 389 us; 4, 16, 32 passes 436, 412, 433 us; work-groups that stay resident and
-        // stride over the rows 432 us).
-        p.wg_rows = 8 * C::RPB;
+        // stride over the rows 432 us).  A launch has fewer than 2^32 threads: of more rows (2^32 of one channel) more to a work-group.
+        constexpr long long kMost = (1ll << 32) / C::THREADS - 1;
+        const long long per = passes <= 8 * kMost ? 8 : (passes + kMost - 1) / kMost;
+        p.wg_rows = per * C::RPB;
         p.wg_step = 0;
-        grid = (passes + 7) / 8;
+        grid = (passes + per - 1) / per;
     } else {
         // Long rows: the work-groups that fit the device at once stride over the rows (16000 rows of 4096: 108 us, of eight
         // rows to a work-group 125 us: the last of them leave the device half empty).
@@ -121,7 +123,6 @@ int launch_rows(NormParams p, hipStream_t stream)
         p.wg_rows = C::RPB;
         p.wg_step = grid * C::RPB;
     }
-    SRHIP_REQUIRE(grid < (1ll << 31), "norm_residual: too many rows");
     hipLaunchKernelGGL((norm_residual_kernel<C, MAPG>), dim3((unsigned)grid), dim3(C::THREADS), 0, stream, p);
     return srhip_check_launch("norm_residual_kernel");
 }

@@ -438,3 +438,29 @@ def test_gates_beyond_one_row_of_the_launch(F, c, gates):
         size = p.abs().sum(1) * (K * a * (1 - a) + 4 * a)
         off[part] = ((got[part] - p.sum(1) * a * (1 - a)).abs() / (size * 2.0 ** -24 + 1e-30)).amax(-1)
     assert float(off.max()) < 2               # once on each side
+
+
+def test_more_rows_than_a_launch_has_work_groups(F):
+    """2^32 rows of one channel and more, forward and backward: the last rows equal those on their own."""
+    rows, tail = (1 << 32) + 4099, 5003
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB")
+    t = torch.randn(tail, 1, generator=torch.Generator().manual_seed(31)).bfloat16().cuda()
+    x = torch.full((rows, 1), 2.0, dtype=torch.bfloat16, device="cuda")
+    x[-tail:] = t
+    w = torch.full((1,), 1.5, device="cuda")
+    how = dict(gate=w, scale=0.5, pre=(w, w), kind="rms")
+    r, n = F.norm_residual(x, x, **how)
+    rt, nt = F.norm_residual(t, t, **how)
+    first = F.norm_residual(x[:8], x[:8], **how)
+    assert torch.equal(r[-tail:], rt) and torch.equal(n[-tail:], nt)
+    for lo in range(0, rows - tail, 1 << 28):
+        part = slice(lo, min(lo + (1 << 28), rows - tail))
+        assert bool((r[part] == first[0][0]).all()) and bool((n[part] == first[1][0]).all()), lo
+    del n
+    g = F.norm_residual_bwd(x, r, x, x, **how)
+    gt = F.norm_residual_bwd(t, rt, t, t, **how)
+    assert torch.equal(g.dx[-tail:], gt.dx) and torch.equal(g.dh[-tail:], gt.dh)
+    del g, r, x
+    torch.cuda.empty_cache()
