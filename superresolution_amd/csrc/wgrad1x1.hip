@@ -241,7 +241,8 @@ SRHIP_API int srhip_wgrad1x1(const void* x, const void* x_scales, const void* dz
     SRHIP_REQUIRE(x_cstride >= cin && x_cstride % per == 0 && dz_cstride >= cout && dz_cstride % 8 == 0,
                   "wgrad1x1: %d and %d channels per pixel (at least the layer's %d and %d, multiples of %d and 8)", x_cstride, dz_cstride, cin, cout, per);
     SRHIP_REQUIRE((((size_t)x | (size_t)dz) & 15) == 0, "wgrad1x1: maps start at multiples of 16 bytes");
-    SRHIP_REQUIRE((long long)cout * cin < (1ll << 30), "wgrad1x1: weight too large");
+    // (a launch has fewer than 2^32 threads: the sums' has 1024 for 64 weights or biases)
+    SRHIP_REQUIRE((long long)cout * (cin + 1ll) < (1ll << 28) - 64, "wgrad1x1: weight too large");
     const PwPlan q = pw_plan(npix, cin, cout);
     SRHIP_REQUIRE(q.runs == 1 || workspace, "wgrad1x1: null workspace");
     PwParams p;
@@ -253,7 +254,7 @@ SRHIP_API int srhip_wgrad1x1(const void* x, const void* x_scales, const void* dz
     p.cin = cin; p.xs = x_cstride; p.xg = srhip_div_up(x_cstride, kCk8Group); p.cout = cout; p.zs = dz_cstride;
     p.nci = q.nci; p.blocks = q.blocks; p.runs = q.runs;
     const long long grid = (long long)srhip_div_up(q.runs, 8) * 8 * q.blocks;
-    SRHIP_REQUIRE(grid < (1ll << 31), "wgrad1x1: layer too large");
+    SRHIP_REQUIRE(grid < (1ll << 32) / kThreads, "wgrad1x1: layer too large");
     hipStream_t s = (hipStream_t)stream;
     if (x_scales) hipLaunchKernelGGL(wgrad1x1_kernel<true>, dim3((unsigned)grid), dim3(kThreads), 0, s, p);
     else hipLaunchKernelGGL(wgrad1x1_kernel<false>, dim3((unsigned)grid), dim3(kThreads), 0, s, p);

@@ -154,3 +154,6 @@ def test_launches_of_too_many_threads_are_refused_on_the_host():
     from superresolution_amd._lib import lib
     # one pixel to a group of 32: 2^26 groups, 2^32 threads
     _refused(lib.srhip_checkpoint8_pack_signbits(P, P, P, P, 1024, 65536, 1, None), "too large")
+    # 2^28 weights: 2^32 threads of the launch that adds the runs (1024 for 64), square or in a row
+    _refused(lib.srhip_wgrad1x1(P, None, P, P, P, P, 1 << 20, 1 << 14, 1 << 14, 1 << 14, 1 << 14, None), "too large")
+    _refused(lib.srhip_wgrad1x1(P, None, P, P, P, P, 64, 1 << 28, 1 << 28, 1, 8, None), "too large")
