@@ -115,9 +115,18 @@ Plan plan_of(const srhip_norm_residual_bwd_args* a)
     if (grid > resident) grid = resident;
     const long long gates = a->gate_mode == SRHIP_GATE_ROWS ? a->rows / a->rows_per_gate : 1;
     const long long per_gate = a->rows / gates;
-    long long segs = (grid + gates - 1) / gates;
-    const long long most = (per_gate + q.rpb - 1) / q.rpb;
-    if (segs > most) segs = most;
+    // Items run in rounds of `grid`, and a round of a few takes as long as a full one: as many items to a gate as r rounds hold, for
+    // the r of the fewest or three more that takes the least passes (an item's sums counted as two), and a further round for a
+    // thirty-second at least.  (64 channels from checkpoints, 1024 work-groups at once: three crops of 1024^2 in 1026 items 614 us, in
+    // 1023 428; seven in 1029 1417, in 1022 983; 600 gates of 3500 rows in 1200 items 389, in 3000 323.)
+    const long long passes_per_gate = (per_gate + q.rpb - 1) / q.rpb, fewest = (gates + grid - 1) / grid;
+    long long segs = 1, least = -1;
+    for (long long r = fewest; r < fewest + 4; ++r) {
+        long long k = r * grid / gates;
+        if (k > passes_per_gate) k = passes_per_gate;
+        const long long cost = r * ((passes_per_gate + k - 1) / k + 2);
+        if (least < 0 || cost < least - least / 32) { least = cost; segs = k; }
+    }
     q.seg_rows = (((per_gate + segs - 1) / segs) + q.rpb - 1) / q.rpb * q.rpb;
     q.segs = (int)((per_gate + q.seg_rows - 1) / q.seg_rows);
     q.items = gates * q.segs;

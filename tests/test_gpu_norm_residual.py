@@ -464,3 +464,25 @@ def test_more_rows_than_a_launch_has_work_groups(F):
     assert torch.equal(g.dx[-tail:], gt.dx) and torch.equal(g.dh[-tail:], gt.dh)
     del g, r, x
     torch.cuda.empty_cache()
+
+
+def test_no_round_of_a_few_items(F):
+    """How the backward pass cuts rows into items, read from the workspace that it asks for (work-groups x 2c sums, items x (2c + 1)): the
+    rounds of items take about the time that the rows would take on all work-groups, for any number of crops and for more gates than
+    work-groups.  (An item more than a round holds would double it.)"""
+    from superresolution_amd._lib import NormResidualBwdArgs, lib
+    c = 64
+
+    def floats(gates, per, **kw):
+        a = NormResidualBwdArgs(rows=gates * per, rows_per_gate=per, c=c, gate_mode=1, **kw)
+        return lib.srhip_norm_residual_bwd_workspace_bytes(a) // 4
+
+    for kw in (dict(dtype=0), dict(dtype=1), dict(dtype=0, h_scales=1, r_scales=1)):
+        most = floats(1, 1 << 24, **kw) // (4 * c + 1)       # work-groups at once: an item each
+        assert most >= 256
+        for per, many, bound in ((1 << 20, range(1, 33), 1.08), (2048, (most // 2 + 88, most + 1, most * 3 // 2, most * 2 + 1), 1.3)):
+            for gates in many:
+                got = floats(gates, per, **kw)
+                items = got // (4 * c + 1) if got <= most * (4 * c + 1) else (got - most * 2 * c) // (2 * c + 1)
+                rounds = -(-items // most)
+                assert rounds * most <= bound * items, (kw, gates, items, most)
