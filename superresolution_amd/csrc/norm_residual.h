@@ -27,7 +27,7 @@ struct Lane {
     int c0[C::V];                    // first channel of a vector
     bool in[C::V];                   // it is in the row
     unsigned e[C::V];                // first element of it, from the first row of the work-group's pass on
-    float counts[C::ODD ? C::E : 1]; // ODD: 1 where the element counts in sums, else 0
+    int shared[C::ODD ? C::V : 1];   // ODD: the leading elements of a vector that do not count in sums (all, behind the row)
     int rg;                          // the lane's row of the pass
     bool whole;                      // every vector of every lane is in the row
     __device__ __forceinline__ Lane(const int c)
@@ -41,13 +41,11 @@ struct Lane {
             in[v] = start < c;
             c0[v] = !in[v] ? 0 : C::ODD && start + C::VEC > c ? c - C::VEC : start;
             e[v] = (unsigned)(rg * c + c0[v]);
-            if constexpr (C::ODD)
-#pragma unroll
-                for (int k = 0; k < C::VEC; ++k) counts[v * C::VEC + k] = in[v] && c0[v] + k >= start ? 1.0f : 0.0f;
+            if constexpr (C::ODD) shared[v] = in[v] ? start - c0[v] : C::VEC;
         }
     }
     // whether element j is this lane's in the sums
-    __device__ __forceinline__ bool mine(const int j) const { return C::ODD ? counts[j] != 0.0f : in[j / C::VEC]; }
+    __device__ __forceinline__ bool mine(const int j) const { return C::ODD ? j % C::VEC >= shared[j / C::VEC] : in[j / C::VEC]; }
 };
 
 // Sums over the TPR lanes of a row; `turn` alternates between two scratch areas, so that one barrier per sum is enough.

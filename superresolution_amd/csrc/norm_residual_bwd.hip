@@ -189,7 +189,6 @@ SRHIP_API int srhip_norm_residual_bwd(const srhip_norm_residual_bwd_args* a, voi
     p.c = a->c; p.groups = srhip_div_up(a->c, kCk8Group); p.layer = a->kind == SRHIP_NORM_LAYER; p.post = a->post; p.pre = a->pre;
     p.gate_mode = a->gate_mode; p.gate_f32 = a->dtype != SRHIP_DT_F32 && a->gate_f32; p.sigmoid = a->gate_sigmoid;
     p.need_h = need_h; p.item_flush = a->dh && (a->post || a->gate_mode == SRHIP_GATE_ROWS || a->dscale);
-    p.direct = q.items == 1;
     p.scale = a->scale; p.eps = a->eps; p.inv_c = 1.0f / (float)a->c;
     const long long gates = p.gate_mode == SRHIP_GATE_ROWS ? a->rows / p.rows_per_gate : 0;
     const hipStream_t s = (hipStream_t)stream;
@@ -198,7 +197,7 @@ SRHIP_API int srhip_norm_residual_bwd(const srhip_norm_residual_bwd_args* a, voi
     const long long gate_rows = gates > gate_row ? (gates + gate_row - 1) / gate_row : 1;
     SRHIP_REQUIRE(gate_rows < (1ll << 16), "norm_residual_bwd: too many gates");
     const int launched = rows(a, &p, q, s);
-    if (launched != SRHIP_OK || p.direct || (!p.pre && !p.item_flush)) return launched;
+    if (launched != SRHIP_OK || q.items == 1 || (!p.pre && !p.item_flush)) return launched;
     hipLaunchKernelGGL(norm_residual_bwd_sums_kernel, dim3((unsigned)((5 + gate_row) * cblocks), (unsigned)gate_rows), dim3(kCols * kParts), 0, s, p, q.grid,
                        cblocks, gates, gate_row);
     return srhip_check_launch("norm_residual_bwd_sums_kernel");

@@ -486,3 +486,17 @@ def test_no_round_of_a_few_items(F):
                 items = got // (4 * c + 1) if got <= most * (4 * c + 1) else (got - most * 2 * c) // (2 * c + 1)
                 rounds = -(-items // most)
                 assert rounds * most <= bound * items, (kw, gates, items, most)
+
+
+@pytest.mark.parametrize("c", [10, 16, 24, 31, 32, 45, 64, 99, 128, 200, 255, 256, 401, 512])
+def test_two_waves_to_a_simd_at_least(F, c):
+    """Rows of up to 512 channels, of either type, from maps and checkpoints, with a gate map (the most registers) and without: two work-groups
+    of four waves fit a CU, read from the workspace that the call asks for."""
+    from superresolution_amd._lib import NormResidualBwdArgs, lib
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    for dtype in (0, 1):
+        for ck in (None, 1):
+            for gate in (0, 2):
+                a = NormResidualBwdArgs(rows=1 << 24, rows_per_gate=1 << 24, c=c, dtype=dtype, gate_mode=gate, h_scales=ck, r_scales=ck)
+                groups = lib.srhip_norm_residual_bwd_workspace_bytes(a) // 4 // (4 * c + 1)
+                assert groups >= 2 * cus * 0.95, (dtype, ck, gate, groups)
