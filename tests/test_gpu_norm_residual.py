@@ -500,3 +500,39 @@ def test_two_waves_to_a_simd_at_least(F, c):
                 a = NormResidualBwdArgs(rows=1 << 24, rows_per_gate=1 << 24, c=c, dtype=dtype, gate_mode=gate, h_scales=ck, r_scales=ck)
                 groups = lib.srhip_norm_residual_bwd_workspace_bytes(a) // 4 // (4 * c + 1)
                 assert groups >= 2 * cus * 0.95, (dtype, ck, gate, groups)
+
+
+FIRST_CALLS = """
+import torch
+from superresolution_amd import functional as F
+c = {c}
+x, h = (torch.randn(9, 5, c, generator=torch.Generator().manual_seed(s)).to({dtype}).cuda() for s in (1, 2))
+w = torch.rand(c, generator=torch.Generator().manual_seed(3)).cuda()
+how = dict(post=(w, None), pre=(w, w), kind="rms")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    r, n = F.norm_residual(x, h, **how)
+    g = F.norm_residual_bwd(h, r, x, h, **how)
+for _ in range(3):
+    for t in (r, n, g.dx, g.dh, g.dpost_weight):
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    want = F.norm_residual(x, h, **how)
+    wg = F.norm_residual_bwd(h, want[0], x, h, **how)
+    assert torch.equal(r, want[0]) and torch.equal(n, want[1])
+    assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(g, wg))
+print("replayed")
+"""
+
+
+@pytest.mark.parametrize("c,dtype", [(1000, "torch.float32"), (2056, "torch.bfloat16")])
+def test_first_call_of_a_process_inside_a_capture(c, dtype):
+    """A process whose first calls are recorded: what the long rows' kernels, forward and backward, ask of the runtime once is asked while the
+    stream is being captured (in this process other tests have asked before)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(c=c, dtype=dtype)], cwd=root, capture_output=True, text=True, timeout=100)
+    assert run.returncode == 0 and "replayed" in run.stdout, (run.returncode, run.stdout, run.stderr[-2000:])
