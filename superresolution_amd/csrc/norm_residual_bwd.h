@@ -30,7 +30,7 @@ struct NormBwdParams {
     float* item_scale;                          // [items]: the item's part of ds
     float *dpost_w, *dpost_b, *dpre_w, *dpre_b, *dscale;
     long long rows, rows_per_gate, seg_rows;    // an item is seg_rows rows of one gate's
-    long long items;                            // one: its work-group writes the results, there is no second launch
+    long long items;
     int segs;                                   // items per gate
     int c, groups, layer, post, pre, gate_mode, gate_f32, sigmoid, need_h, item_flush;
     float scale, eps, inv_c;
@@ -82,33 +82,6 @@ __device__ __forceinline__ void sum_row_groups(float* tile, const Lane<C>& l, co
         }
     }
 }
-// The results of a single item, from the sums that its work-group has just written.  Behind everything else, where no row is held
-// any more: the same writes in the places of the sums cost the kernels 4 to 28 registers, and those of fp32 rows of odd width with a
-// gate map their second wave to a SIMD (3 x 135 x 241 rows of 99: 106 us instead of 74, from checkpoints 94 instead of 68).
-__device__ __forceinline__ void finish_item()
-{
-    // the kernel's argument once more, at an address that says nothing of it: its members are loaded here, not kept since the start
-    auto args = (const __attribute__((address_space(4))) NormBwdParams*)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(args));
-    const NormBwdParams& p = *(const NormBwdParams*)args;
-    const float scale = p.scale_ptr ? *p.scale_ptr : p.scale;
-    __syncthreads();
-    for (int ch = threadIdx.x; ch < p.c; ch += blockDim.x) {
-        float slope;
-        const float gv = gate_value(p, 0, ch, slope);
-        if (p.pre) {
-            p.dpre_w[ch] = p.wg_sums[ch];
-            if (p.dpre_b) p.dpre_b[ch] = p.wg_sums[p.c + ch];
-        }
-        if (!p.item_flush) continue;
-        const float a1 = p.item_sums[ch], a0 = p.item_sums[p.c + ch];
-        if (p.dpost_w) p.dpost_w[ch] = scale * (gv * a1);
-        if (p.dpost_b) p.dpost_b[ch] = scale * (gv * a0);
-        if (p.gate_mode == SRHIP_GATE_ROWS) ((float*)p.dgate)[ch] = gate_gradient(p, ch, scale * slope, a1, a0);
-    }
-    if (p.dscale && threadIdx.x == 0) *p.dscale = *p.item_scale;
-}
-
 template <class C>
 constexpr int row_groups_tile() { return C::RPB == 1 ? C::THREADS / 64 : C::CMAX * (C::TPR <= 64 ? C::THREADS / 64 : C::RPB); }
 
@@ -185,11 +158,14 @@ struct RawRow {
 // registers left alone, and at 128, nine of them spilled, 64 channels of four crops take 587 us instead of 617), three with a
 // gate map (two crops: 469 us instead of 532; of fp32 maps 138 us instead of 74, they are left alone), else what the compiler
 // arrives at (the same on maps: 684 us for 681).
-template <class C, bool CK, bool MAPG>
-constexpr int min_waves() { return C::SIZE == 2 && C::TPR <= 64 ? (MAPG ? 3 : CK ? 4 : 1) : 1; }
+template <class C, bool CK, bool MAPG, bool SINGLE>
+constexpr int min_waves() { return C::SIZE == 2 && C::TPR <= 64 && !SINGLE ? (MAPG ? 3 : CK ? 4 : 1) : 1; }
 
-template <class C, bool CK, bool MAPG>
-__global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG>())) void norm_residual_bwd_kernel(const NormBwdParams p)
+// SINGLE: a few rows, one item; its work-group writes the results and there is no second launch.  A kernel of its own: in the others
+// these writes cost 4 to 28 registers, and fp32 rows of odd width with a gate map their second wave to a SIMD (3 x 135 x 241 rows
+// of 99: 106 us instead of 73, from checkpoints 94 instead of 68).
+template <class C, bool CK, bool MAPG, bool SINGLE>
+__global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG, SINGLE>())) void norm_residual_bwd_kernel(const NormBwdParams p)
 {
     constexpr int SIZE = C::SIZE, VEC = C::VEC, E = C::E;
     __shared__ float scratch[row_sum_scratch<C>()];
@@ -317,12 +293,19 @@ __global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG>())) void norm_r
                 const float gv = gate_value(p, s, ch, slope);
                 out[ch] = v;
                 if (p.dscale) part += v * gv * (p.post_w ? p.post_w[ch] : 1.0f);
+                if constexpr (SINGLE)
+                    if (p.dpost_w) p.dpost_w[ch] = scale * (gv * v);
             });
             sum_row_groups<C>(tile, l, a0, p.c, [&](const int ch, const float v) {
                 float slope;
                 const float gv = gate_value(p, s, ch, slope);
                 out[p.c + ch] = v;
                 if (p.dscale && p.post_b) part += v * gv * p.post_b[ch];
+                if constexpr (SINGLE) {
+                    if (p.dpost_b) p.dpost_b[ch] = scale * (gv * v);
+                    if (p.gate_mode == SRHIP_GATE_ROWS)   // out[ch] is this thread's own
+                        ((float*)p.dgate)[ch] = gate_gradient(p, ch, scale * slope, out[ch], v);
+                }
             });
             if (p.dscale) {
                 part = lanes_sum<64>(part);
@@ -331,17 +314,19 @@ __global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG>())) void norm_r
                 __syncthreads();
                 if (threadIdx.x == 0) {
                     for (int k = 1; k < C::THREADS / 64; ++k) part += tile[k];
-                    p.item_scale[item] = part;
+                    *(SINGLE ? p.dscale : p.item_scale + item) = part;
                 }
             }
         }
     }
     if (p.pre) {
         float* out = p.wg_sums + (long long)blockIdx.x * 2 * p.c;
-        sum_row_groups<C>(tile, l, a_w, p.c, [&](const int ch, const float v) { out[ch] = v; });
-        sum_row_groups<C>(tile, l, a_b, p.c, [&](const int ch, const float v) { out[p.c + ch] = v; });
+        sum_row_groups<C>(tile, l, a_w, p.c, [&](const int ch, const float v) { (SINGLE ? p.dpre_w : out)[ch] = v; });
+        sum_row_groups<C>(tile, l, a_b, p.c, [&](const int ch, const float v) {
+            if (!SINGLE) out[p.c + ch] = v;
+            else if (p.dpre_b) p.dpre_b[ch] = v;
+        });
     }
-    if (p.items == 1) finish_item();
 }
 
 // How the rows are cut into items and work-groups
@@ -376,7 +361,7 @@ void shape_of(Plan& q)
     const int dev = srhip_current_device();
     int n = fit[dev].load(std::memory_order_relaxed);
     if (n == 0) {
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, norm_residual_bwd_kernel<C, CK, MAPG>, C::THREADS, 0) != hipSuccess || n < 1) n = 1;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, norm_residual_bwd_kernel<C, CK, MAPG, false>, C::THREADS, 0) != hipSuccess || n < 1) n = 1;
         fit[dev].store(n, std::memory_order_relaxed);
     }
     q.grid = n;
@@ -390,7 +375,8 @@ int shape_or_launch(const NormBwdParams* p, Plan& q, hipStream_t stream)
         shape_of<C, CK, MAPG>(q);
         return SRHIP_OK;
     }
-    hipLaunchKernelGGL((norm_residual_bwd_kernel<C, CK, MAPG>), dim3(q.grid), dim3(C::THREADS), 0, stream, *p);
+    if (q.items == 1) hipLaunchKernelGGL((norm_residual_bwd_kernel<C, CK, MAPG, true>), dim3(1), dim3(C::THREADS), 0, stream, *p);
+    else hipLaunchKernelGGL((norm_residual_bwd_kernel<C, CK, MAPG, false>), dim3(q.grid), dim3(C::THREADS), 0, stream, *p);
     return srhip_check_launch("norm_residual_bwd_kernel");
 }
 template <class T, bool ODD>
