@@ -597,7 +597,7 @@ SRHIP_API int srhip_layernorm_cf_bwd_f32_static(const float* x, const float* wei
  * ------------------------------------------------------------------------- */
 SRHIP_API int srhip_checkpoint8_pack(const void* x, int dtype /* SRHIP_DT_* */, void* codes, void* scales, long long rows, int c, void* stream);
 /* The same for an (n, h, w, 64) bf16 map, also writing its ReLU pattern as srhip_signbits_from_map_bf16 does
- * (srhip_conv3x3_signbits_bytes(n, h, w) bytes). */
+ * (srhip_conv3x3_signbits_bytes(n, h, w) bytes, below 2^34). */
 SRHIP_API int srhip_checkpoint8_pack_signbits(const void* x, void* codes, void* scales, void* signbits, int n, int h, int w, void* stream);
 SRHIP_API int srhip_checkpoint8_restore(const void* codes, const void* scales, void* y, int dtype, long long rows, int c, void* stream);
 /* out = dy where the code is a positive number, else 0 (bf16; out may be dy). */
@@ -614,7 +614,7 @@ SRHIP_API int srhip_conv_wgrad_checkpoint8(const srhip_wgrad_job* jobs, const vo
  *   dw[co][ci] = sum dz[pixel][co] * x[pixel][ci]  (fp32 (cout, cin)),  db[co] = sum dz[pixel][co]  (db may be NULL)
  * x: bf16 pixels of x_cstride channels, or (x_scales not NULL) a checkpoint's codes; dz: bf16 pixels of dz_cstride channels.
  * x_cstride is a multiple of 8 (16: codes), dz_cstride of 8; both maps start at multiples of 16 bytes; channels behind cin, cout
- * are not used.  workspace: srhip_wgrad1x1_workspace_bytes(npix, cin, cout) bytes (none: NULL).  Written, not accumulated;
+ * are not used; cout * (cin + 1) stays below 2^28 - 64.  workspace: srhip_wgrad1x1_workspace_bytes(npix, cin, cout) bytes (none: NULL).  Written, not accumulated;
  * deterministic.  From codes the result is that of the restored map, bit for bit. */
 SRHIP_API size_t srhip_wgrad1x1_workspace_bytes(long long npix, int cin, int cout);
 SRHIP_API int srhip_wgrad1x1(const void* x, const void* x_scales, const void* dz, float* dw, float* db, void* workspace, long long npix,

@@ -295,7 +295,8 @@ class _ConvAuto(Function):
 def _auto_wgrad(srcs, dzs: Tensor, w: Tensor):
     """Weight and bias gradient of a layer of ``_ConvAuto`` from the gradient of its (equivalent stride-1) pre-activation:
     the MFMA weight-gradient kernel per (<= 64 input, <= 64 output) channel slice pair (a GEMM over a million pixels with a
-    160 x 160 output is a shape the GEMM library serves three times slower than that)."""
+    160 x 160 output is a shape the GEMM library serves three times slower than that).  1x1 layers too:
+    functional.conv_wgrad's pixel GEMM adds in another order, these gradients keep theirs."""
     cout, cin, k, _ = w.shape
     return F_._conv_wgrad(srcs, dzs, cin, cout, k)
 

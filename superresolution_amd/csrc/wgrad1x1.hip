@@ -13,7 +13,8 @@
 // The runs' partial blocks (fp32) are added by a second launch in a fixed order; a single run writes the result.
 // Measured from checkpoints, beside the centre tap of conv3x3_wgrad.hip with its 64 x 64 slice pairs: 160 -> 112 channels, 65 k
 // pixels 21 us (49), a million 109 us = 3.6 TB/s (262); 256 -> 192, a million 204 us = 3.3 TB/s (485).  Short maps are bound by
-// the two launches (16 us), long ones by the LDS traffic of the operand reads beside HBM.
+// their few dependent steps and the partial sums (65 k pixels: nine steps and 16 MB, 16 us, and 5 us for the launch that adds
+// them), long ones by the LDS traffic of the operand reads beside HBM.
 #include "rows_util.h"
 
 namespace {
