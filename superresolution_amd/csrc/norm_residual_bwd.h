@@ -332,7 +332,7 @@ __global__ __launch_bounds__(C::THREADS, (min_waves<C, CK, MAPG, SINGLE>())) voi
 // How the rows are cut into items and work-groups
 struct Plan {
     long long items, seg_rows;
-    int segs, grid, rpb, threads;
+    int segs, grid, rpb;
 };
 
 // Calls f with the configuration of a row of c channels: the narrowest group of lanes that holds it.
@@ -353,7 +353,7 @@ int with_rows(const int c, F&& f)
     return f(RowCfg<RowVec<T>, 512, 2 * K, ODD>{});
 }
 
-// How many work-groups of the call's kernel a CU holds, and their shape; asked of the runtime once per kernel and device.
+// How many work-groups of the call's kernel a CU holds, and their rows; asked of the runtime once per kernel and device.
 template <class C, bool CK, bool MAPG>
 void shape_of(Plan& q)
 {
@@ -366,7 +366,6 @@ void shape_of(Plan& q)
     }
     q.grid = n;
     q.rpb = C::RPB;
-    q.threads = C::THREADS;
 }
 template <class C, bool CK, bool MAPG>
 int shape_or_launch(const NormBwdParams* p, Plan& q, hipStream_t stream)

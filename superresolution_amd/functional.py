@@ -396,8 +396,8 @@ WGRAD_MERGE_PIXELS = 1 << 18
 def conv_wgrad(srcs, dz: torch.Tensor, cin: int, cout: int, ksize: int):
     """Weight and bias gradient (dw (cout,cin,ksize,ksize), db (cout,), fp32) of a stride-1 layer with kernel 1 or 3 and any
     channel counts, whose input is the concatenation of ``srcs`` (NHWC bf16 maps of a multiple of 8 channels or their checkpoints,
-    of 16), from the gradient dz of its pre-activation output.  A pointwise layer of one source is a GEMM over the pixels (srhip_wgrad1x1); otherwise one job
-    per (<= 64 input, <= 64 output) channel slice pair, the channel windows read in place."""
+    of 16), from the gradient dz of its pre-activation output.  A pointwise layer of one source is a GEMM over the pixels
+    (srhip_wgrad1x1); otherwise one job per (<= 64 input, <= 64 output) channel slice pair, the channel windows read in place."""
     if ksize == 1 and len(srcs) == 1:
         return _wgrad1x1(srcs[0], dz, cin, cout)
     return _conv_wgrad(srcs, dz, cin, cout, ksize, len(srcs) == 1 and dz.numel() // max(1, dz.shape[-1]) <= WGRAD_MERGE_PIXELS)
